@@ -230,6 +230,44 @@ int nk_fused_compile_grad(nk_ctx* ctx, int32_t dtype, int32_t n_inputs, int32_t 
 int nk_fused_run_grad(nk_ctx* ctx, nk_fused* f, int32_t rank, nk_buf* grad, const int32_t* cfg_grad, nk_buf* err, const int32_t* cfg_err,
                       nk_buf* const* srcs, const int32_t* const* cfgs);
 
+/* ---- a feed-forward sub-layer: layer norm, dropout, the gated block (no counterpart in the reference) ----
+ * F32 and F64. Operands are views like everywhere else; each call takes what it needs beside them from the device's memory pool in the
+ * order of ctx's stream and gives it back, so that calls on several contexts, or captured into several graphs, share nothing. A drain's
+ * elements must be distinct (no virtual drain), and a drain may not overlap another operand unless said otherwise. */
+
+/* Layer norm over the last dim (n = its extent; a row = the elements that share all other indices): mu = mean(src), v = mean((src - mu)^2),
+ * drn = (src - mu) / sqrt(v + eps) * gain + shift. gain and shift are views of RANK 1 with n elements, either may be NULL (1 and 0); eps >= 0.
+ * stats: NULL, or a buffer of at least 2 * rows elements that receives every row's mu and then every row's 1 / sqrt(v + eps), rows in
+ * row-major order -- what the backward pass reads. drn may be src itself (the same view). Sums are taken in the call's type, v from the
+ * differences to mu; the result does not depend on scheduling. */
+int nk_layer_norm(nk_ctx* ctx, int32_t dtype, int32_t rank, nk_buf* drn, const int32_t* cfg0, nk_buf* src, const int32_t* cfg1,
+                  nk_buf* gain, const int32_t* cfg_gain, nk_buf* shift, const int32_t* cfg_shift, double eps, nk_buf* stats);
+/* Its gradients for the error err of the result (any of the three drains may be NULL): with xh = (src - mu) / sqrt(v + eps) and g = err * gain
+ * dsrc = (g - mean(g) - xh * mean(g * xh)) / sqrt(v + eps), dgain = sum over the rows of err * xh, dshift = sum over the rows of err
+ * (views of rank 1 with n elements). err may be virtual; dsrc may be err itself. stats is what the forward call left there. */
+int nk_layer_norm_grad(nk_ctx* ctx, int32_t dtype, int32_t rank, nk_buf* dsrc, const int32_t* cfg_dsrc, nk_buf* dgain, const int32_t* cfg_dgain,
+                       nk_buf* dshift, const int32_t* cfg_dshift, nk_buf* err, const int32_t* cfg_err, nk_buf* src, const int32_t* cfg1,
+                       nk_buf* gain, const int32_t* cfg_gain, nk_buf* stats);
+
+/* Dropout: drn = keep ? src * (1 / (1 - p)) : 0, plus residual where that is not NULL; 0 <= p < 1. The element with row-major index i of the
+ * shape is dropped when word i % 4 of Philox4x32-10 (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", 2011) for the counter
+ * (i / 4 as 64 bits, stream as 64 bits, low words first) and the key seed is below floor(p * 2^32). The mask is a function of (seed,
+ * stream, i) alone and is never stored: the backward pass is the same call on the error, whatever the views are. Calls with
+ * one seed and different streams draw independent masks. A dropped element is 0 even where src is not finite. drn may be src or residual itself. */
+int nk_dropout(nk_ctx* ctx, int32_t dtype, int32_t rank, nk_buf* drn, const int32_t* cfg0, nk_buf* src, const int32_t* cfg1,
+               nk_buf* residual, const int32_t* cfg2, double p, int64_t seed, int64_t stream);
+
+/* Gated feed-forward block: drn = f(src @ w_gate) * (src @ w_up) for src [T, D], w_gate and w_up [D, H], drn [T, H]; all of rank 2. fun: one of
+ * NK_FUN_SIG, SILU, GELU, RELU, TANH, IDY (NK_ERR_UNSUPPORTED for the others). kept: NULL, or a buffer of at least 2 * T * H elements that
+ * receives src @ w_gate and then src @ w_up, row-major -- what the backward pass reads. */
+int nk_gated(nk_ctx* ctx, int32_t fun, int32_t dtype, nk_buf* drn, const int32_t* cfg0, nk_buf* src, const int32_t* cfg1,
+             nk_buf* w_gate, const int32_t* cfg_gate, nk_buf* w_up, const int32_t* cfg_up, nk_buf* kept);
+/* Its gradients for the error err of the result (any of the three drains may be NULL): with g, u = kept, dg = err * u * f'(g), du = err * f(g)
+ * dsrc = dg @ w_gate^T + du @ w_up^T, dw_gate = src^T @ dg, dw_up = src^T @ du. err may be virtual. */
+int nk_gated_grad(nk_ctx* ctx, int32_t fun, int32_t dtype, nk_buf* dsrc, const int32_t* cfg_dsrc, nk_buf* dw_gate, const int32_t* cfg_dgate,
+                  nk_buf* dw_up, const int32_t* cfg_dup, nk_buf* err, const int32_t* cfg_err, nk_buf* src, const int32_t* cfg1,
+                  nk_buf* w_gate, const int32_t* cfg_gate, nk_buf* w_up, const int32_t* cfg_up, nk_buf* kept);
+
 /* ---- ordering between contexts (no reference counterpart: OpenCLDevice owns a single in-order queue) ----
  * A second nk_ctx on the same device is a second stream. An event recorded on one context's stream can be waited
  * for by another's, e.g. to let copies of finished results run beside the next computation. Waiting for an event

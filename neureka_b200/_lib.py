@@ -30,6 +30,7 @@ FUN_IDS = [
     "quad", "relu", "selu", "silu", "sig", "sin", "softplus", "softsign", "sqrt", "tanh", "fast_tanh",
 ]
 FUN = {name: i for i, name in enumerate(FUN_IDS)}
+GATES = ("sig", "silu", "gelu", "relu", "tanh", "idy")   # the functions nk_gated takes
 OPS = {"+": NK_OP_ADD, "-": NK_OP_SUB, "*": NK_OP_MUL, "/": NK_OP_DIV, "%": NK_OP_MOD, "**": NK_OP_POW}
 
 
@@ -92,6 +93,11 @@ SIGNATURES = {
     "nk_sum": (C.c_int, [_vp, _i32, _i32, _vp, _cfg, _vp, _i64]),
     "nk_arg_reduce": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _cfg, _vp, _i64]),
     "nk_sum_static": (C.c_int, [_vp, _i32, _i32, _vp, _cfg, _vp, _i64]),
+    "nk_layer_norm": (C.c_int, [_vp, _i32, _i32, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp, _cfg, _dbl, _vp]),
+    "nk_layer_norm_grad": (C.c_int, [_vp, _i32, _i32, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp]),
+    "nk_dropout": (C.c_int, [_vp, _i32, _i32, _vp, _cfg, _vp, _cfg, _vp, _cfg, _dbl, _i64, _i64]),
+    "nk_gated": (C.c_int, [_vp, _i32, _i32, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp]),
+    "nk_gated_grad": (C.c_int, [_vp, _i32, _i32, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp, _cfg, _vp]),
     "nk_set_conv_path": (C.c_int, [_vp, _i32]),
     "nk_last_conv_path": (C.c_int, [_vp, C.POINTER(_i32)]),
     "nk_last_kernel": (C.c_char_p, [_vp]),

@@ -12,6 +12,8 @@ ADAction recipes (reference file:line):
    product is reduced to the operand's shape (handle*drain summed over the broadcast dims), the mathematical
    gradient, using the same reduction kernel.
  * sumItems: the scalar error becomes a virtual tensor of the input's shape (algorithms/SumAlgorithm.java:29-33)
+ * layer norm, dropout, the gated block (no counterpart in the reference): one call gives the errors of all tracked operands; dropout's is
+   the same call on the error, which draws the same mask again
  * gradient accumulation: g <- g + e = one "+" kernel and one assign kernel (math/Functions.java:74,
    TensorImpl.java:1275-1300)
 """
@@ -181,6 +183,58 @@ def extreme(x: Tensor, want_max: bool) -> Tensor:
             dev.access(g).write(value).at(g.ndconf.index_of_index(index))
             return g
         out.graph_node = GraphNode(out, [(x, action)])
+    return out
+
+
+class _Joint:
+    """The errors of an operation's operands that one kernel call computes together: made when the backward pass asks for the first one,
+    handed out one after the other, gone with the last."""
+
+    def __init__(self, operands, compute: Callable[[Tensor, List[bool]], List[Optional[Tensor]]]):
+        self._wanted = [t is not None and _tracks(t) for t in operands]
+        self._compute = compute
+        self._ready: List[Optional[Tensor]] = []
+        indices = [i for i, w in enumerate(self._wanted) if w]
+        self.parents = [(operands[i], lambda err, i=i: self._take(i, err, i == indices[0], i == indices[-1])) for i in indices]
+
+    def _take(self, i: int, err: Tensor, first: bool, last: bool) -> Tensor:
+        if first:
+            self._ready = self._compute(err, self._wanted)
+        e = self._ready[i]
+        if last:
+            self._ready = []
+        return e
+
+
+def layer_norm(x: Tensor, gain: Optional[Tensor], shift: Optional[Tensor], eps: float) -> Tensor:
+    tracked = any(t is not None and _tracks(t) for t in (x, gain, shift))
+    out, stats = F.run_layer_norm(x, gain, shift, eps, tracked)
+    if tracked:
+        stats.is_intermediate = False
+        joint = _Joint((x, gain, shift), lambda err, wanted: F.run_layer_norm_gradients(err, x, gain, shift, stats, wanted))
+        out.graph_node = GraphNode(out, joint.parents)
+    return out
+
+
+def dropout(x: Tensor, p: float, seed: int, stream: int, residual: Optional[Tensor]) -> Tensor:
+    out = F.run_dropout(x, p, seed, stream, residual)
+    parents = []
+    if _tracks(x):
+        parents.append((x, lambda err: F.run_dropout(err, p, seed, stream)))
+    if residual is not None and _tracks(residual):
+        parents.append((residual, lambda err: err))
+    if parents:
+        out.graph_node = GraphNode(out, parents)
+    return out
+
+
+def gated(x: Tensor, w_gate: Tensor, w_up: Tensor, fun: str) -> Tensor:
+    tracked = any(_tracks(t) for t in (x, w_gate, w_up))
+    out, kept = F.run_gated(x, w_gate, w_up, fun, tracked)
+    if tracked:
+        kept.is_intermediate = False
+        joint = _Joint((x, w_gate, w_up), lambda err, wanted: F.run_gated_gradients(err, x, w_gate, w_up, kept, fun, wanted))
+        out.graph_node = GraphNode(out, joint.parents)
     return out
 
 

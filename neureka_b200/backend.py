@@ -32,6 +32,7 @@ SCALAR_BROADCAST = "ScalarBroadcast"
 SUM_ALGORITHM = "SumAlgorithm"
 MIN_ALGORITHM, MAX_ALGORITHM = "min_algorithm", "max_algorithm"
 DOT_ALGORITHM = "DotProductAlgorithm"
+LAYER_NORM, DROPOUT, GATED = "LayerNorm", "Dropout", "GatedProduct"   # (no counterpart in the reference)
 
 OPERATORS = ["**", "/", "*", "%", "-", "+"]                       # Power ... Addition
 CONV_OPS = ["x", "«x", "x»"]                            # Convolution, XConvLeft, XConvRight
@@ -272,6 +273,101 @@ class CudaReduce(ImplementationFor):
         return out
 
 
+def _cfg_vector(t: Tensor):
+    """_cfg of a tensor whose axes but the last have extent 1, as a view of rank 1."""
+    c = t.ndconf
+    if c.rank == 1:
+        return _cfg(t)
+    base = sum(o * s for o, s in zip(c.offset, c.strides))
+    arr = np.array((c.shape[-1], 1, 1, base, c.strides[-1] * c.spread[-1]), dtype=np.int32)
+    return arr, arr.ctypes.data_as(C.POINTER(C.c_int32))
+
+
+def _buf_cfg(t: Optional[Tensor], cfg=_cfg):
+    """An operand as the C ABI takes it -- buffer, descriptor, and the array that backs the descriptor -- or nothing at all."""
+    if t is None:
+        return None, None, None
+    keep, c = cfg(t)
+    return t._data.buf, c, keep
+
+
+class CudaLayerNorm(ImplementationFor):
+    """Drain, source[, gain][, shift][, statistics]; args: which of them are there, eps."""
+
+    def run(self, call: ExecutionCall) -> Tensor:
+        dev, a = call.device, call.args
+        t0, t1 = call.input(0), call.input(1)
+        gain, shift, stats = a["gain"], a["shift"], a["stats"]
+        for t in call.inputs[1:]:
+            t.set_is_virtual(False)
+        dt = _same_type(call, call.arity)
+        k0, c0 = _cfg(t0); k1, c1 = _cfg(t1)
+        bg, cg, kg = _buf_cfg(gain, _cfg_vector); bs, cs, ks = _buf_cfg(shift, _cfg_vector)
+        L.check(L.lib.nk_layer_norm(dev.ctx, dt, t0.rank, t0._data.buf, c0, t1._data.buf, c1, bg, cg, bs, cs, a["eps"],
+                                    None if stats is None else stats._data.buf), dev.ctx)
+        t0.version += 1
+        return t0
+
+
+class CudaLayerNormGradients(ImplementationFor):
+    """Error, source, statistics[, gain] and the drains that are wanted; args: dsrc, dgain, dshift, gain, stats."""
+
+    def run(self, call: ExecutionCall) -> Tensor:
+        dev, a = call.device, call.args
+        err, src, gain, stats = call.input(0), call.input(1), a["gain"], a["stats"]
+        dt = _same_type(call, call.arity)
+        ke, ce = _cfg_virtual(err); k1, c1 = _cfg(src)
+        b0, c0, k0 = _buf_cfg(a["dsrc"]); bg, cg, kg = _buf_cfg(gain, _cfg_vector)
+        bdg, cdg, kdg = _buf_cfg(a["dgain"], _cfg_vector); bds, cds, kds = _buf_cfg(a["dshift"], _cfg_vector)
+        L.check(L.lib.nk_layer_norm_grad(dev.ctx, dt, src.rank, b0, c0, bdg, cdg, bds, cds, err._data.buf, ce, src._data.buf, c1, bg, cg, stats._data.buf), dev.ctx)
+        return err
+
+
+class CudaDropout(ImplementationFor):
+    """Drain, source[, residual]; args: p, seed, stream."""
+
+    def run(self, call: ExecutionCall) -> Tensor:
+        dev, a = call.device, call.args
+        t0, t1 = call.input(0), call.input(1)
+        residual = call.input(2) if call.arity == 3 else None
+        dt = _same_type(call, call.arity)
+        k0, c0 = _cfg(t0); k1, c1 = _cfg_virtual(t1)
+        br, cr, kr = _buf_cfg(residual, _cfg_virtual)
+        L.check(L.lib.nk_dropout(dev.ctx, dt, t0.rank, t0._data.buf, c0, t1._data.buf, c1, br, cr, a["p"], a["seed"], a["stream"]), dev.ctx)
+        t0.version += 1
+        return t0
+
+
+class CudaGated(ImplementationFor):
+    """Drain, source, gate's and up's weights[, kept products]; args: fun."""
+
+    def run(self, call: ExecutionCall) -> Tensor:
+        dev = call.device
+        t0, x, wg, wu = call.inputs[:4]
+        for t in (x, wg, wu):
+            t.set_is_virtual(False)
+        dt = _same_type(call, call.arity)
+        k0, c0 = _cfg(t0); k1, c1 = _cfg(x); k2, c2 = _cfg(wg); k3, c3 = _cfg(wu)
+        L.check(L.lib.nk_gated(dev.ctx, L.FUN[call.args["fun"]], dt, t0._data.buf, c0, x._data.buf, c1, wg._data.buf, c2, wu._data.buf, c3,
+                               call.input(4)._data.buf if call.arity == 5 else None), dev.ctx)
+        t0.version += 1
+        return t0
+
+
+class CudaGatedGradients(ImplementationFor):
+    """Error, source, weights, kept products and the drains that are wanted; args: fun, dsrc, dgate, dup."""
+
+    def run(self, call: ExecutionCall) -> Tensor:
+        dev, a = call.device, call.args
+        err, x, wg, wu, kept = call.inputs[:5]
+        dt = _same_type(call, call.arity)
+        ke, ce = _cfg_virtual(err); k1, c1 = _cfg(x); k2, c2 = _cfg(wg); k3, c3 = _cfg(wu)
+        b0, c0, k0 = _buf_cfg(a["dsrc"]); bg, cg, kg = _buf_cfg(a["dgate"]); bu, cu, ku = _buf_cfg(a["dup"])
+        L.check(L.lib.nk_gated_grad(dev.ctx, L.FUN[a["fun"]], dt, b0, c0, bg, cg, bu, cu, err._data.buf, ce, x._data.buf, c1, wg._data.buf, c2, wu._data.buf, c3,
+                                    kept._data.buf), dev.ctx)
+        return err
+
+
 class CudaBackend:
     """BackendExtension for the CUDA device (src/main/java/neureka/backend/api/BackendExtension.java:15-70).
 
@@ -305,6 +401,9 @@ class CudaBackend:
         # DotProduct (linear/DotProduct.java; CLDot / CPUDot): two vectors of one length are the `x` call whose single dim
         # is summed away -- the convolution implementation serves it (its long-reduction kernel)
         self._set("dot", DOT_ALGORITHM, CudaConvolution())
+        self._set("layerNorm", LAYER_NORM, CudaLayerNorm())
+        self._set("dropout", DROPOUT, CudaDropout())
+        self._set("gated", GATED, CudaGated())
 
     def implementation_for(self, operation: str, algorithm: str) -> ImplementationFor:
         try:

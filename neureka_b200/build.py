@@ -45,6 +45,9 @@ SOURCES = [
     ("nk_fused.cu", ["-I", OBJDIR]),
     ("nk_group.cu", []),
     ("nk_reduce.cu", []),
+    ("nk_norm.cu", []),
+    ("nk_dropout.cu", ["-fmad=false"]),
+    ("nk_gated.cu", ["-fmad=false"]),
     ("nk_probe.cu", []),
     ("nk_sum_static.cu", ["-fmad=false"]),
     ("nk_jrand.cpp", ["-Xcompiler", "-ffp-contract=off"]),

@@ -1,0 +1,114 @@
+// Dropout from a counter-based generator (no counterpart in the reference). The mask of element i is a function of (seed, stream, i): word i % 4 of
+// Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011) for the counter (i / 4, stream) and
+// the key seed. It is drawn where it is needed, forward and backward, and never stored.
+//
+// A thread takes four consecutive elements, the four words of one counter. Compiled with -fmad=false: the product and the residual's sum
+// round one after the other, like the separate operators.
+#include "nk_internal.h"
+
+namespace {
+
+struct DropPlan {
+    int nd;
+    int64_t total;
+    int64_t ext[NK_MAX_RANK];
+    int64_t s0[NK_MAX_RANK], s1[NK_MAX_RANK], s2[NK_MAX_RANK];   // drain, source, residual
+    unsigned below;                                              // words below this are dropped
+    unsigned key[2], stream[2];
+};
+
+__device__ __forceinline__ void philox(unsigned (&c)[4], unsigned k0, unsigned k1) {
+#pragma unroll
+    for (int r = 0; r < 10; r++) {
+        const unsigned a_lo = c[0] * 0xD2511F53u, a_hi = __umulhi(c[0], 0xD2511F53u);
+        const unsigned b_lo = c[2] * 0xCD9E8D57u, b_hi = __umulhi(c[2], 0xCD9E8D57u);
+        c[0] = b_hi ^ c[1] ^ (k0 + unsigned(r) * 0x9E3779B9u);
+        c[1] = b_lo;
+        c[2] = a_hi ^ c[3] ^ (k1 + unsigned(r) * 0xBB67AE85u);
+        c[3] = a_lo;
+    }
+}
+
+// Any views: the indices of the first element by division, the next three by counting up.
+template <class T, bool RES>
+__global__ void __launch_bounds__(256) nk_dropout_kernel(T* out, const T* src, const T* res, const DropPlan p, const T scale) {
+    const int64_t groups = (p.total + 3) / 4, stride = int64_t(gridDim.x) * blockDim.x;
+    for (int64_t g = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; g < groups; g += stride) {
+        unsigned c[4] = {unsigned(g), unsigned(uint64_t(g) >> 32), p.stream[0], p.stream[1]};
+        philox(c, p.key[0], p.key[1]);
+        int64_t idx[NK_MAX_RANK], rem = g * 4, o0 = 0, o1 = 0, o2 = 0;
+        for (int k = p.nd - 1; k >= 0; k--) {
+            const int64_t q = rem / p.ext[k];
+            idx[k] = rem - q * p.ext[k];
+            rem = q;
+            o0 += idx[k] * p.s0[k]; o1 += idx[k] * p.s1[k]; o2 += idx[k] * p.s2[k];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (g * 4 + j < p.total) {
+                T v = c[j] >= p.below ? src[o1] * scale : T(0);
+                if (RES) v = res[o2] + v;
+                out[o0] = v;
+            }
+            for (int k = p.nd - 1; k >= 0; k--) {
+                idx[k]++; o0 += p.s0[k]; o1 += p.s1[k]; o2 += p.s2[k];
+                if (idx[k] < p.ext[k]) break;
+                o0 -= idx[k] * p.s0[k]; o1 -= idx[k] * p.s1[k]; o2 -= idx[k] * p.s2[k];
+                idx[k] = 0;
+            }
+        }
+    }
+}
+
+template <class T>
+int launch(nk_ctx* ctx, T* out, const T* src, const T* res, const DropPlan& p, double prob) {
+    const T scale = T(1.0 / (1.0 - prob));
+    const int grid = nk_grid_for(ctx, (p.total + 3) / 4, 256, 8);
+    if (res) nk_dropout_kernel<T, true><<<grid, 256, 0, ctx->stream>>>(out, src, res, p, scale);
+    else nk_dropout_kernel<T, false><<<grid, 256, 0, ctx->stream>>>(out, src, res, p, scale);
+    return nk_after_launch(ctx, "nk_dropout_kernel");
+}
+
+}  // namespace
+
+extern "C" int nk_dropout(nk_ctx* ctx, int32_t dtype, int32_t rank, nk_buf* drn, const int32_t* cfg0, nk_buf* src, const int32_t* cfg1,
+                          nk_buf* residual, const int32_t* cfg2, double prob, int64_t seed, int64_t stream) {
+    NK_CHECK_CTX(ctx);
+    if (dtype != NK_F32 && dtype != NK_F64) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_dropout: dtype %d not supported (F32/F64 only)", dtype);
+    if (!(prob >= 0.0 && prob < 1.0)) return nk_fail(ctx, NK_ERR_BAD_ARG, "nk_dropout: probability %g outside [0, 1)", prob);
+    NkView v0, v1, v2;
+    int st;
+    if ((st = nk_view_parse(ctx, "nk_dropout(drain)", drn, cfg0, rank, dtype, &v0))) return st;
+    if ((st = nk_check_drain(ctx, "nk_dropout", v0))) return st;
+    if ((st = nk_view_parse(ctx, "nk_dropout(src)", src, cfg1, rank, dtype, &v1))) return st;
+    v2 = v1;
+    if (residual && (st = nk_view_parse(ctx, "nk_dropout(residual)", residual, cfg2, rank, dtype, &v2))) return st;
+    for (int k = 0; k < rank; k++)
+        if (v0.shape[k] != v1.shape[k] || v0.shape[k] != v2.shape[k])
+            return nk_fail(ctx, NK_ERR_BAD_ARG, "nk_dropout: shapes differ at dim %d (%lld, %lld, %lld)", k, (long long)v0.shape[k], (long long)v1.shape[k],
+                           (long long)v2.shape[k]);
+    // size-1 dims go, neighbours merge where every operand is linear across them; the row-major index of an element stays what it is
+    DropPlan p;
+    memset(&p, 0, sizeof(p));
+    p.total = v0.size;
+    for (int k = 0; k < rank; k++) {
+        const int64_t e = v0.shape[k], a = v0.estride[k], b = v1.estride[k], c = residual ? v2.estride[k] : 0;
+        if (e == 1) continue;
+        const int l = p.nd - 1;
+        if (l >= 0 && p.s0[l] == e * a && p.s1[l] == e * b && p.s2[l] == e * c) {
+            p.ext[l] *= e;
+            p.s0[l] = a; p.s1[l] = b; p.s2[l] = c;
+        } else {
+            p.ext[p.nd] = e;
+            p.s0[p.nd] = a; p.s1[p.nd] = b; p.s2[p.nd] = c;
+            p.nd++;
+        }
+    }
+    if (p.nd == 0) { p.nd = 1; p.ext[0] = 1; }
+    p.below = unsigned(prob * 4294967296.0);
+    p.key[0] = unsigned(uint64_t(seed)); p.key[1] = unsigned(uint64_t(seed) >> 32);
+    p.stream[0] = unsigned(uint64_t(stream)); p.stream[1] = unsigned(uint64_t(stream) >> 32);
+    if (dtype == NK_F32)
+        return launch<float>(ctx, (float*)drn->ptr + v0.base, (const float*)src->ptr + v1.base, residual ? (const float*)residual->ptr + v2.base : nullptr, p, prob);
+    return launch<double>(ctx, (double*)drn->ptr + v0.base, (const double*)src->ptr + v1.base, residual ? (const double*)residual->ptr + v2.base : nullptr, p, prob);
+}

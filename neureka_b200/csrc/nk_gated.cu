@@ -1,0 +1,236 @@
+// The gated feed-forward block (no counterpart in the reference):
+//   g = x Wg, u = x Wu, y = f(g) * u;   dg = e * u * f'(g), du = e * f(g), dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du.
+// f and f' are the framework's own functions (nk_scalarfun.cuh, which wants -fmad=false; the products below say fma).
+//
+// nk_gated_tile_kernel: any sizes, any strides, both types. Both products of a tile share the panel of x and end in the same thread, so the
+// activation and the product with it happen in registers.
+#include "nk_gated.h"
+#include "nk_scalarfun.cuh"
+
+namespace {
+
+template <class T>
+__device__ __forceinline__ T gate_fun(int f, bool derive, T x) {
+    switch (f) {
+        case NK_FUN_SIG: return nkf::fun(NK_FUN_SIG, derive, x);
+        case NK_FUN_SILU: return nkf::fun(NK_FUN_SILU, derive, x);
+        case NK_FUN_GELU: return nkf::fun(NK_FUN_GELU, derive, x);
+        case NK_FUN_RELU: return nkf::fun(NK_FUN_RELU, derive, x);
+        case NK_FUN_TANH: return nkf::fun(NK_FUN_TANH, derive, x);
+        default: return nkf::fun(NK_FUN_IDY, derive, x);
+    }
+}
+
+// ---- the tile kernel -------------------------------------------------------------------------------------------------------------
+// FORWARD: C_i = A_0 B_i, out_0 = f(C_0) * C_1 (C_i kept where wanted).  TWO: out_i = A_0 B_i.  SUM: out_0 = A_0 B_0 + A_1 B_1.
+enum { GATED_FORWARD, GATED_TWO, GATED_SUM };
+struct GatedTile {
+    int fun;
+    int64_t M, N, K;
+    GatedMatrix a[2], b[2], out[2];   // [M, K], [K, N], [M, N]
+    void *gate, *up;                  // FORWARD: row-major [M, N] or null
+};
+constexpr int GT = 64, GK = 16;       // 64 x 64 of out, panels of 16 k; 256 threads with 4 x 4 elements of each product
+
+template <class T, int MODE>
+__global__ void __launch_bounds__(256) nk_gated_tile_kernel(const GatedTile p) {
+    constexpr int NB = MODE == GATED_SUM ? 1 : 2, PHASES = MODE == GATED_SUM ? 2 : 1;
+    __shared__ T As[GK][GT + 1], Bs[NB][GK][GT + 1];
+    const int64_t tiles_n = (p.N + GT - 1) / GT;
+    const int64_t m0 = (blockIdx.x / tiles_n) * GT, n0 = (blockIdx.x % tiles_n) * GT;
+    const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+    T acc[NB][4][4];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[b][i][j] = T(0);
+    for (int phase = 0; phase < PHASES; phase++) {
+        const GatedMatrix& A = p.a[phase];
+        for (int64_t k0 = 0; k0 < p.K; k0 += GK) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {   // lanes along the contiguous direction
+                const int e = tid + i * 256, k = A.cs == 1 ? e & 15 : e >> 6, r = A.cs == 1 ? e >> 4 : e & 63;
+                As[k][r] = m0 + r < p.M && k0 + k < p.K ? static_cast<const T*>(A.ptr)[(m0 + r) * A.rs + (k0 + k) * A.cs] : T(0);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const GatedMatrix& B = p.b[MODE == GATED_SUM ? phase : b];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int e = tid + i * 256, k = B.rs == 1 ? e & 15 : e >> 6, c = B.rs == 1 ? e >> 4 : e & 63;
+                    Bs[b][k][c] = n0 + c < p.N && k0 + k < p.K ? static_cast<const T*>(B.ptr)[(k0 + k) * B.rs + (n0 + c) * B.cs] : T(0);
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < GK; k++) {
+                T a[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) a[i] = As[k][ty + 16 * i];
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const T v = Bs[b][k][tx + 16 * j];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[b][i][j] = fma(a[i], v, acc[b][i][j]);
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int64_t m = m0 + ty + 16 * i;
+        if (m >= p.M) continue;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int64_t n = n0 + tx + 16 * j;
+            if (n >= p.N) continue;
+            if (MODE == GATED_FORWARD) {
+                if (p.gate) {
+                    static_cast<T*>(p.gate)[m * p.N + n] = acc[0][i][j];
+                    static_cast<T*>(p.up)[m * p.N + n] = acc[NB - 1][i][j];
+                }
+                static_cast<T*>(p.out[0].ptr)[m * p.out[0].rs + n * p.out[0].cs] = gate_fun<T>(p.fun, false, acc[0][i][j]) * acc[NB - 1][i][j];
+            } else {
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+                    if (p.out[b].ptr) static_cast<T*>(p.out[b].ptr)[m * p.out[b].rs + n * p.out[b].cs] = acc[b][i][j];
+            }
+        }
+    }
+}
+template <class T, int MODE>
+int launch_tiles(nk_ctx* ctx, const GatedTile& p) {
+    const int64_t tiles = ((p.M + GT - 1) / GT) * ((p.N + GT - 1) / GT);
+    if (tiles > 0x7fffffffLL) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_gated: a result of %lld x %lld elements is too large", (long long)p.M, (long long)p.N);
+    nk_gated_tile_kernel<T, MODE><<<unsigned(tiles), 256, 0, ctx->stream>>>(p);
+    return nk_after_launch(ctx, "nk_gated_tile_kernel");
+}
+
+// dg and du, row-major [T, H]
+template <class T>
+__global__ void __launch_bounds__(256) nk_gated_errors_kernel(const GatedCall p, T* __restrict__ dg, T* __restrict__ du) {
+    const int64_t total = p.T * p.H;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t t = i / p.H, h = i - t * p.H;
+        const T e = static_cast<const T*>(p.err.ptr)[t * p.err.rs + h * p.err.cs], g = static_cast<const T*>(p.gate)[i], u = static_cast<const T*>(p.up)[i];
+        dg[i] = e * u * gate_fun<T>(p.fun, true, g);
+        du[i] = e * gate_fun<T>(p.fun, false, g);
+    }
+}
+
+GatedMatrix turned(const GatedMatrix& m) { return GatedMatrix{m.ptr, m.cs, m.rs}; }
+
+template <class T>
+int forward(nk_ctx* ctx, const GatedCall& c) {
+    GatedTile p;
+    memset(&p, 0, sizeof(p));
+    p.fun = c.fun;
+    p.M = c.T; p.N = c.H; p.K = c.D;
+    p.a[0] = c.x;
+    p.b[0] = c.w[0]; p.b[1] = c.w[1];
+    p.out[0] = c.y;
+    p.gate = c.gate; p.up = c.up;
+    return launch_tiles<T, GATED_FORWARD>(ctx, p);
+}
+template <class T>
+int backward(nk_ctx* ctx, const GatedCall& c) {
+    NkWorkspace ws(ctx);
+    int st = ws.get(size_t(c.T) * c.H * 2 * sizeof(T));
+    if (st) return st;
+    T *dg = static_cast<T*>(ws.ptr), *du = dg + c.T * c.H;
+    nk_gated_errors_kernel<T><<<nk_grid_for(ctx, c.T * c.H, 256, 8), 256, 0, ctx->stream>>>(c, dg, du);
+    if ((st = nk_after_launch(ctx, "nk_gated_errors_kernel"))) return st;
+    const GatedMatrix mg{dg, c.H, 1}, mu{du, c.H, 1};
+    GatedTile p;
+    memset(&p, 0, sizeof(p));
+    if (c.dx.ptr) {
+        p.M = c.T; p.N = c.D; p.K = c.H;
+        p.a[0] = mg; p.a[1] = mu;
+        p.b[0] = turned(c.w[0]); p.b[1] = turned(c.w[1]);
+        p.out[0] = c.dx;
+        if ((st = launch_tiles<T, GATED_SUM>(ctx, p))) return st;
+    }
+    if (!c.dw[0].ptr && !c.dw[1].ptr) return NK_OK;
+    p.M = c.D; p.N = c.H; p.K = c.T;
+    p.a[0] = turned(c.x);
+    p.b[0] = mg; p.b[1] = mu;
+    p.out[0] = c.dw[0]; p.out[1] = c.dw[1];
+    return launch_tiles<T, GATED_TWO>(ctx, p);
+}
+
+// One of a call's matrices: a view of rank 2, T / D / H filled in or compared.
+int gated_matrix(nk_ctx* ctx, const char* who, const char* what, nk_buf* buf, const int32_t* cfg, int32_t dtype, bool drain, int64_t* rows, int64_t* cols, GatedMatrix* out) {
+    NkView v;
+    int st;
+    if ((st = nk_view_parse(ctx, who, buf, cfg, 2, dtype, &v))) return st;
+    if (drain && (st = nk_check_drain(ctx, who, v))) return st;
+    if (*rows == 0) *rows = v.shape[0];
+    if (*cols == 0) *cols = v.shape[1];
+    if (v.shape[0] != *rows || v.shape[1] != *cols)
+        return nk_fail(ctx, NK_ERR_BAD_ARG, "%s: %s is [%lld, %lld], expected [%lld, %lld]", who, what, (long long)v.shape[0], (long long)v.shape[1], (long long)*rows, (long long)*cols);
+    out->ptr = static_cast<char*>(buf->ptr) + v.base * int64_t(nk_dtype_size(dtype));
+    out->rs = v.estride[0];
+    out->cs = v.estride[1];
+    return NK_OK;
+}
+int gated_kept(nk_ctx* ctx, const char* who, nk_buf* kept, int32_t dtype, GatedCall* c) {
+    if (kept->magic != 0x4e4b4246) return nk_fail(ctx, NK_ERR_BAD_ARG, "%s: invalid handle of the kept products' buffer", who);
+    if (kept->dtype != dtype || kept->device != ctx->device) return nk_fail(ctx, NK_ERR_BAD_ARG, "%s: the kept products' buffer is of another type or device", who);
+    if (kept->n_elems / 2 / c->H < c->T)
+        return nk_fail(ctx, NK_ERR_BOUNDS, "%s: the kept products need 2 * %lld * %lld elements, the buffer holds %lld", who, (long long)c->T, (long long)c->H, (long long)kept->n_elems);
+    c->gate = kept->ptr;
+    c->up = static_cast<char*>(kept->ptr) + size_t(c->T) * c->H * nk_dtype_size(dtype);
+    return NK_OK;
+}
+int gated_check(nk_ctx* ctx, const char* who, int32_t fun, int32_t dtype) {
+    if (dtype != NK_F32 && dtype != NK_F64) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "%s: dtype %d not supported (F32/F64 only)", who, dtype);
+    if (fun < 0 || fun >= NK_FUN_COUNT) return nk_fail(ctx, NK_ERR_BAD_ARG, "%s: unknown function id %d", who, fun);
+    if (fun != NK_FUN_SIG && fun != NK_FUN_SILU && fun != NK_FUN_GELU && fun != NK_FUN_RELU && fun != NK_FUN_TANH && fun != NK_FUN_IDY)
+        return nk_fail(ctx, NK_ERR_UNSUPPORTED, "%s: function id %d is no gate (sig, silu, gelu, relu, tanh, idy)", who, fun);
+    return NK_OK;
+}
+
+}  // namespace
+
+extern "C" int nk_gated(nk_ctx* ctx, int32_t fun, int32_t dtype, nk_buf* drn, const int32_t* cfg0, nk_buf* src, const int32_t* cfg1, nk_buf* w_gate,
+                        const int32_t* cfg_gate, nk_buf* w_up, const int32_t* cfg_up, nk_buf* kept) {
+    NK_CHECK_CTX(ctx);
+    int st;
+    if ((st = gated_check(ctx, "nk_gated", fun, dtype))) return st;
+    GatedCall c;
+    memset(&c, 0, sizeof(c));
+    c.fun = fun;
+    if ((st = gated_matrix(ctx, "nk_gated(src)", "src", src, cfg1, dtype, false, &c.T, &c.D, &c.x))) return st;
+    if ((st = gated_matrix(ctx, "nk_gated(w_gate)", "w_gate", w_gate, cfg_gate, dtype, false, &c.D, &c.H, &c.w[0]))) return st;
+    if ((st = gated_matrix(ctx, "nk_gated(w_up)", "w_up", w_up, cfg_up, dtype, false, &c.D, &c.H, &c.w[1]))) return st;
+    if ((st = gated_matrix(ctx, "nk_gated(drain)", "the drain", drn, cfg0, dtype, true, &c.T, &c.H, &c.y))) return st;
+    if (kept && (st = gated_kept(ctx, "nk_gated", kept, dtype, &c))) return st;
+    return dtype == NK_F32 ? forward<float>(ctx, c) : forward<double>(ctx, c);
+}
+
+extern "C" int nk_gated_grad(nk_ctx* ctx, int32_t fun, int32_t dtype, nk_buf* dsrc, const int32_t* cfg_dsrc, nk_buf* dw_gate, const int32_t* cfg_dgate, nk_buf* dw_up,
+                             const int32_t* cfg_dup, nk_buf* err, const int32_t* cfg_err, nk_buf* src, const int32_t* cfg1, nk_buf* w_gate, const int32_t* cfg_gate,
+                             nk_buf* w_up, const int32_t* cfg_up, nk_buf* kept) {
+    NK_CHECK_CTX(ctx);
+    int st;
+    if ((st = gated_check(ctx, "nk_gated_grad", fun, dtype))) return st;
+    if (!kept) return nk_fail(ctx, NK_ERR_BAD_ARG, "nk_gated_grad: the products that the forward call kept are needed");
+    GatedCall c;
+    memset(&c, 0, sizeof(c));
+    c.fun = fun;
+    if ((st = gated_matrix(ctx, "nk_gated_grad(src)", "src", src, cfg1, dtype, false, &c.T, &c.D, &c.x))) return st;
+    if ((st = gated_matrix(ctx, "nk_gated_grad(w_gate)", "w_gate", w_gate, cfg_gate, dtype, false, &c.D, &c.H, &c.w[0]))) return st;
+    if ((st = gated_matrix(ctx, "nk_gated_grad(w_up)", "w_up", w_up, cfg_up, dtype, false, &c.D, &c.H, &c.w[1]))) return st;
+    if ((st = gated_matrix(ctx, "nk_gated_grad(err)", "err", err, cfg_err, dtype, false, &c.T, &c.H, &c.err))) return st;
+    if (dsrc && (st = gated_matrix(ctx, "nk_gated_grad(dsrc)", "dsrc", dsrc, cfg_dsrc, dtype, true, &c.T, &c.D, &c.dx))) return st;
+    if (dw_gate && (st = gated_matrix(ctx, "nk_gated_grad(dw_gate)", "dw_gate", dw_gate, cfg_dgate, dtype, true, &c.D, &c.H, &c.dw[0]))) return st;
+    if (dw_up && (st = gated_matrix(ctx, "nk_gated_grad(dw_up)", "dw_up", dw_up, cfg_dup, dtype, true, &c.D, &c.H, &c.dw[1]))) return st;
+    if ((st = gated_kept(ctx, "nk_gated_grad", kept, dtype, &c))) return st;
+    if (!dsrc && !dw_gate && !dw_up) return NK_OK;
+    return dtype == NK_F32 ? backward<float>(ctx, c) : backward<double>(ctx, c);
+}

@@ -86,6 +86,30 @@ struct NkView {
 // Parses + validates cfg against buf. Returns a status; on error the message is stored in ctx.
 int nk_view_parse(nk_ctx* ctx, const char* who, const nk_buf* buf, const int32_t* cfg, int rank, int dtype, NkView* out);
 
+// Device memory for the length of one call: from the pool in the order of ctx's stream, back to it when the call returns (work queued by
+// then keeps its block). Unlike ctx->scratch nothing outlives the call, so two captured graphs, or a graph and an eager call, never share it.
+struct NkWorkspace {
+    nk_ctx* ctx;
+    void* ptr = nullptr;
+    explicit NkWorkspace(nk_ctx* c) : ctx(c) {}
+    NkWorkspace(const NkWorkspace&) = delete;
+    NkWorkspace& operator=(const NkWorkspace&) = delete;
+    ~NkWorkspace() {
+        if (ptr) cudaFreeAsync(ptr, ctx->stream);
+    }
+    int get(size_t bytes) {
+        NK_CUDA(ctx, cudaMallocAsync(&ptr, bytes, ctx->stream));
+        return NK_OK;
+    }
+};
+
+// A drain whose elements are not distinct would be written by several threads at once.
+inline int nk_check_drain(nk_ctx* ctx, const char* who, const NkView& v) {
+    for (int k = 0; k < v.rank; k++)
+        if (v.shape[k] > 1 && v.estride[k] == 0) return nk_fail(ctx, NK_ERR_BAD_ARG, "%s: dim %d of the drain maps several indices to one element", who, k);
+    return NK_OK;
+}
+
 inline int nk_grid_for(const nk_ctx* ctx, int64_t work_items, int block, int ctas_per_sm) {
     int64_t need = (work_items + block - 1) / block;
     int64_t cap = int64_t(ctx->prop.multiProcessorCount) * ctas_per_sm;

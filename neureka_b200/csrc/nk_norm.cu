@@ -1,0 +1,412 @@
+// Layer norm over the last dim, forward and backward (no counterpart in the reference).
+//
+//   mu = mean(x), v = mean((x - mu)^2), r = 1 / sqrt(v + eps), xh = (x - mu) * r, y = xh * gain + shift
+//   g = e * gain:  dx = r * (g - mean(g) - xh * mean(g * xh)),  dgain = sum over rows of e * xh,  dshift = sum over rows of e
+//
+// Every sum is taken in the tensor's type over a fixed partition of the row (or column), so the result does not depend on scheduling; v
+// comes from the differences to a mean that is known before (no difference of large sums).
+#include "nk_internal.h"
+
+namespace {
+
+template <class T, int W> struct NormVec { using type = T; };
+template <> struct NormVec<float, 4> { using type = float4; };
+template <> struct NormVec<double, 2> { using type = double2; };
+template <class T> constexpr int norm_w() { return 16 / int(sizeof(T)); }
+
+// The rows of a call: what the outer dims come to after merging, with a stride per operand and dim.
+struct NormPlan {
+    int nd;                                  // outer dims, at least 1
+    int64_t rows, n;
+    int64_t ext[NK_MAX_RANK];
+    int64_t s[3][NK_MAX_RANK], inner[3];     // 0: drain, 1: source, 2: error; strides of the outer dims and of the normalised one
+    int64_t gain_s, shift_s;                 // strides of gain and shift
+};
+
+template <int OP>
+__device__ __forceinline__ int64_t norm_row(const NormPlan& p, int64_t r) {
+    int64_t off = 0;
+    for (int k = p.nd - 1; k > 0; k--) {
+        const int64_t q = r / p.ext[k];
+        off += (r - q * p.ext[k]) * p.s[OP][k];
+        r = q;
+    }
+    return off + r * p.s[OP][0];
+}
+// W elements from column c on; past n: zeros (W divides n where W > 1)
+template <class T, int W>
+__device__ __forceinline__ void norm_load(const T* row, int64_t c, int64_t inner, int64_t n, T (&v)[W]) {
+    if (W > 1) {
+        if (c < n) *reinterpret_cast<typename NormVec<T, W>::type*>(v) = *reinterpret_cast<const typename NormVec<T, W>::type*>(row + c);
+        else {
+#pragma unroll
+            for (int k = 0; k < W; k++) v[k] = T(0);
+        }
+    } else v[0] = c < n ? row[c * inner] : T(0);
+}
+template <class T, int W>
+__device__ __forceinline__ void norm_store(T* row, int64_t c, int64_t inner, int64_t n, const T (&v)[W]) {
+    if (c >= n) return;
+    if (W > 1) *reinterpret_cast<typename NormVec<T, W>::type*>(row + c) = *reinterpret_cast<const typename NormVec<T, W>::type*>(v);
+    else row[c * inner] = v[0];
+}
+
+constexpr int NORM_THREADS = 256;
+// sum over the CTA, the same value in every thread
+template <class T>
+__device__ __forceinline__ T norm_cta_sum(T v, T* smem) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int warp = threadIdx.x >> 5;
+    __syncthreads();   // smem may still be read from the sum before
+    if ((threadIdx.x & 31) == 0) smem[warp] = v;
+    __syncthreads();
+    v = smem[0];
+#pragma unroll
+    for (int w = 1; w < NORM_THREADS / 32; w++) v += smem[w];
+    return v;
+}
+
+// ---- rows of any length: cut into chunks of NORM_THREADS * W * 8 elements, a CTA per chunk ---------------------------------------
+constexpr int NORM_NV = 8;
+
+// mean and sum of squared differences to it, per chunk: part[(row * chunks + chunk) * 2]
+template <class T, int W>
+__global__ void __launch_bounds__(NORM_THREADS) nk_norm_chunk_stats_kernel(const T* __restrict__ src, T* __restrict__ part, const NormPlan p, int64_t chunks) {
+    __shared__ T smem[NORM_THREADS / 32];
+    constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
+    for (int64_t u = blockIdx.x; u < p.rows * chunks; u += gridDim.x) {
+        const int64_t row = u / chunks, c0 = (u - row * chunks) * L, left = p.n - c0 < L ? p.n - c0 : L;
+        const T* x = src + norm_row<1>(p, row);
+        T v[NORM_NV][W], sum = T(0);
+#pragma unroll
+        for (int k = 0; k < NORM_NV; k++) {
+            norm_load<T, W>(x, c0 + (k * NORM_THREADS + threadIdx.x) * W, p.inner[1], p.n, v[k]);
+#pragma unroll
+            for (int j = 0; j < W; j++) sum += v[k][j];
+        }
+        const T mean = norm_cta_sum(sum, smem) / T(left);
+        T m2 = T(0);
+#pragma unroll
+        for (int k = 0; k < NORM_NV; k++)
+#pragma unroll
+            for (int j = 0; j < W; j++)
+                if (c0 + (k * NORM_THREADS + threadIdx.x) * W + j < p.n) m2 += (v[k][j] - mean) * (v[k][j] - mean);
+        m2 = norm_cta_sum(m2, smem);
+        if (threadIdx.x == 0) { part[2 * u] = mean; part[2 * u + 1] = m2; }
+    }
+}
+// The row's mean and variance from its chunks': mu = sum(n_i mean_i) / n, v = sum(m2_i + n_i (mean_i - mu)^2) / n; then the chunk's results.
+template <class T, int W>
+__global__ void __launch_bounds__(NORM_THREADS) nk_norm_chunk_apply_kernel(T* out, const T* src, const T* __restrict__ part, const T* __restrict__ gain,
+                                                                           const T* __restrict__ shift, T* __restrict__ stats, const NormPlan p, int64_t chunks, T eps) {
+    __shared__ T smem[NORM_THREADS / 32];
+    constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
+    for (int64_t u = blockIdx.x; u < p.rows * chunks; u += gridDim.x) {
+        const int64_t row = u / chunks, chunk = u - row * chunks, c0 = chunk * L;
+        auto length = [&](int64_t i) { return T(i + 1 < chunks ? L : p.n - i * L); };
+        T sum = T(0);
+        for (int64_t i = threadIdx.x; i < chunks; i += NORM_THREADS) sum += length(i) * part[2 * (row * chunks + i)];
+        const T mean = norm_cta_sum(sum, smem) / T(p.n);
+        T m2 = T(0);
+        for (int64_t i = threadIdx.x; i < chunks; i += NORM_THREADS) {
+            const T d = part[2 * (row * chunks + i)] - mean;
+            m2 += part[2 * (row * chunks + i) + 1] + length(i) * d * d;
+        }
+        const T rstd = T(1) / sqrt(norm_cta_sum(m2, smem) / T(p.n) + eps);
+        if (stats && chunk == 0 && threadIdx.x == 0) { stats[row] = mean; stats[p.rows + row] = rstd; }
+        const T* x = src + norm_row<1>(p, row);
+        T* y = out + norm_row<0>(p, row);
+#pragma unroll
+        for (int k = 0; k < NORM_NV; k++) {
+            const int64_t c = c0 + (k * NORM_THREADS + threadIdx.x) * W;
+            T v[W];
+            norm_load<T, W>(x, c, p.inner[1], p.n, v);
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                v[j] = (v[j] - mean) * rstd;
+                if (c + j < p.n) {
+                    if (gain) v[j] *= gain[(c + j) * p.gain_s];
+                    if (shift) v[j] += shift[(c + j) * p.shift_s];
+                }
+            }
+            norm_store<T, W>(y, c, p.inner[0], p.n, v);
+        }
+    }
+}
+
+// sum(g) and sum(g * xh), per chunk
+template <class T, int W>
+__global__ void __launch_bounds__(NORM_THREADS) nk_norm_chunk_sums_kernel(const T* __restrict__ err, const T* __restrict__ src, const T* __restrict__ gain,
+                                                                          const T* __restrict__ stats, T* __restrict__ part, const NormPlan p, int64_t chunks) {
+    __shared__ T smem[NORM_THREADS / 32];
+    constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
+    for (int64_t u = blockIdx.x; u < p.rows * chunks; u += gridDim.x) {
+        const int64_t row = u / chunks, c0 = (u - row * chunks) * L;
+        const T *x = src + norm_row<1>(p, row), *e = err + norm_row<2>(p, row);
+        const T mean = stats[row], rstd = stats[p.rows + row];
+        T s1 = T(0), s2 = T(0);
+#pragma unroll
+        for (int k = 0; k < NORM_NV; k++) {
+            const int64_t c = c0 + (k * NORM_THREADS + threadIdx.x) * W;
+            T xv[W], ev[W];
+            norm_load<T, W>(x, c, p.inner[1], p.n, xv);
+            norm_load<T, W>(e, c, p.inner[2], p.n, ev);
+#pragma unroll
+            for (int j = 0; j < W; j++)
+                if (c + j < p.n) {
+                    const T g = gain ? ev[j] * gain[(c + j) * p.gain_s] : ev[j];
+                    s1 += g;
+                    s2 += g * ((xv[j] - mean) * rstd);
+                }
+        }
+        s1 = norm_cta_sum(s1, smem);
+        s2 = norm_cta_sum(s2, smem);
+        if (threadIdx.x == 0) { part[2 * u] = s1; part[2 * u + 1] = s2; }
+    }
+}
+// the chunks' sums to the row's means, a warp per row: means[row], means[rows + row]
+template <class T>
+__global__ void __launch_bounds__(NORM_THREADS) nk_norm_row_means_kernel(const T* __restrict__ part, T* __restrict__ means, int64_t rows, int64_t chunks, T n) {
+    const int lane = threadIdx.x & 31;
+    for (int64_t row = int64_t(blockIdx.x) * (NORM_THREADS / 32) + (threadIdx.x >> 5); row < rows; row += int64_t(gridDim.x) * (NORM_THREADS / 32)) {
+        T s1 = T(0), s2 = T(0);
+        for (int64_t i = lane; i < chunks; i += 32) { s1 += part[2 * (row * chunks + i)]; s2 += part[2 * (row * chunks + i) + 1]; }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { s1 += __shfl_xor_sync(0xffffffffu, s1, o); s2 += __shfl_xor_sync(0xffffffffu, s2, o); }
+        if (lane == 0) { means[row] = s1 / n; means[rows + row] = s2 / n; }
+    }
+}
+// A thread owns W columns and walks a group of rows: dx, and the group's part of the column sums, cols[(group * 2 + which) * n + column].
+template <class T, int W>
+__global__ void __launch_bounds__(NORM_THREADS) nk_norm_columns_kernel(T* out, const T* err, const T* src, const T* __restrict__ gain, const T* __restrict__ stats,
+                                                                       const T* __restrict__ means, T* __restrict__ cols, const NormPlan p, int64_t groups, int64_t per) {
+    const int64_t blocks_c = (p.n + NORM_THREADS * W - 1) / (NORM_THREADS * W);
+    for (int64_t u = blockIdx.x; u < blocks_c * groups; u += gridDim.x) {
+        const int64_t group = u / blocks_c, c = ((u - group * blocks_c) * NORM_THREADS + threadIdx.x) * W;
+        if (c >= p.n) continue;
+        const int64_t r1 = (group + 1) * per < p.rows ? (group + 1) * per : p.rows;
+        T gv[W], sg[W], ss[W];
+#pragma unroll
+        for (int j = 0; j < W; j++) { gv[j] = gain ? gain[(c + j) * p.gain_s] : T(1); sg[j] = ss[j] = T(0); }
+        for (int64_t row = group * per; row < r1; row++) {
+            const T mean = stats[row], rstd = stats[p.rows + row];
+            T xv[W], ev[W];
+            norm_load<T, W>(src + norm_row<1>(p, row), c, p.inner[1], p.n, xv);
+            norm_load<T, W>(err + norm_row<2>(p, row), c, p.inner[2], p.n, ev);
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                const T xh = (xv[j] - mean) * rstd;
+                sg[j] += ev[j] * xh;
+                ss[j] += ev[j];
+                if (out) xv[j] = rstd * (ev[j] * gv[j] - means[row] - xh * means[p.rows + row]);
+            }
+            if (out) norm_store<T, W>(out + norm_row<0>(p, row), c, p.inner[0], p.n, xv);
+        }
+        if (cols) {
+            norm_store<T, W>(cols + (group * 2) * p.n, c, 1, p.n, sg);
+            norm_store<T, W>(cols + (group * 2 + 1) * p.n, c, 1, p.n, ss);
+        }
+    }
+}
+// the groups' parts of the column sums, added in group order
+template <class T>
+__global__ void __launch_bounds__(NORM_THREADS) nk_norm_columns_finish_kernel(T* dgain, int64_t dgain_s, T* dshift, int64_t dshift_s, const T* __restrict__ cols, int64_t n,
+                                                                              int64_t groups) {
+    for (int64_t c = int64_t(blockIdx.x) * NORM_THREADS + threadIdx.x; c < n; c += int64_t(gridDim.x) * NORM_THREADS) {
+        T sg = T(0), ss = T(0);
+        for (int64_t g = 0; g < groups; g++) { sg += cols[(g * 2) * n + c]; ss += cols[(g * 2 + 1) * n + c]; }
+        if (dgain) dgain[c * dgain_s] = sg;
+        if (dshift) dshift[c * dshift_s] = ss;
+    }
+}
+
+// ---- host side -----------------------------------------------------------------------------------------------------------------
+// The outer dims of up to three views of one shape, size-1 dims dropped, neighbours merged where every operand is linear across them.
+void norm_plan(const NkView* const (&v)[3], NormPlan* p) {
+    memset(p, 0, sizeof(*p));
+    const NkView& shape = *v[1];
+    p->rows = 1;
+    for (int k = 0; k + 1 < shape.rank; k++) {
+        const int64_t e = shape.shape[k];
+        p->rows *= e;
+        if (e == 1) continue;
+        const int l = p->nd - 1;
+        bool merge = l >= 0;
+        for (int t = 0; t < 3 && merge; t++) merge = !v[t] || p->s[t][l] == e * v[t]->estride[k];
+        const int at = merge ? l : p->nd++;
+        p->ext[at] = merge ? p->ext[at] * e : e;
+        for (int t = 0; t < 3; t++) p->s[t][at] = v[t] ? v[t]->estride[k] : 0;
+    }
+    if (p->nd == 0) { p->nd = 1; p->ext[0] = 1; }
+    p->n = shape.shape[shape.rank - 1];
+    for (int t = 0; t < 3; t++) p->inner[t] = v[t] ? v[t]->estride[shape.rank - 1] : 1;
+}
+// 16-byte accesses along the rows of operand t
+template <class T>
+bool norm_vec(const NormPlan& p, int t, const T* base) {
+    if (p.inner[t] != 1 || p.n % norm_w<T>() || reinterpret_cast<uintptr_t>(base) % 16) return false;
+    for (int k = 0; k < p.nd; k++)
+        if (p.s[t][k] % norm_w<T>()) return false;
+    return true;
+}
+
+template <class T, int W>
+int forward_w(nk_ctx* ctx, T* out, const T* src, const T* gain, const T* shift, T* stats, const NormPlan& p, T eps) {
+    constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
+    const int64_t chunks = (p.n + L - 1) / L;
+    NkWorkspace ws(ctx);
+    int st = ws.get(size_t(p.rows) * chunks * 2 * sizeof(T));
+    if (st) return st;
+    T* part = static_cast<T*>(ws.ptr);
+    const int grid = nk_grid_for(ctx, p.rows * chunks, 1, 32);
+    nk_norm_chunk_stats_kernel<T, W><<<grid, NORM_THREADS, 0, ctx->stream>>>(src, part, p, chunks);
+    if ((st = nk_after_launch(ctx, "nk_norm_chunk_stats_kernel"))) return st;
+    nk_norm_chunk_apply_kernel<T, W><<<grid, NORM_THREADS, 0, ctx->stream>>>(out, src, part, gain, shift, stats, p, chunks, eps);
+    return nk_after_launch(ctx, "nk_norm_chunk_apply_kernel");
+}
+template <class T>
+int forward(nk_ctx* ctx, T* out, const T* src, const T* gain, const T* shift, T* stats, const NormPlan& p, double eps) {
+    if (norm_vec(p, 0, out) && norm_vec(p, 1, src)) return forward_w<T, norm_w<T>()>(ctx, out, src, gain, shift, stats, p, T(eps));
+    return forward_w<T, 1>(ctx, out, src, gain, shift, stats, p, T(eps));
+}
+
+template <class T>
+struct NormGrad {
+    T *out, *dgain, *dshift;
+    const T *err, *src, *gain, *stats;
+    int64_t dgain_s, dshift_s;
+};
+template <class T, int W>
+int backward_w(nk_ctx* ctx, const NormGrad<T>& a, const NormPlan& p) {
+    constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
+    const int64_t chunks = (p.n + L - 1) / L, blocks_c = (p.n + NORM_THREADS * W - 1) / (NORM_THREADS * W);
+    const bool cols = a.dgain || a.dshift;
+    // row groups: as many as fill the chip, at most one per row
+    int64_t groups = (int64_t(ctx->prop.multiProcessorCount) * 8 + blocks_c - 1) / blocks_c;
+    if (groups > p.rows) groups = p.rows;
+    const int64_t per = (p.rows + groups - 1) / groups;
+    groups = (p.rows + per - 1) / per;
+    auto pad = [](size_t b) { return (b + 255) / 256 * 256; };
+    const size_t part_bytes = pad(size_t(p.rows) * chunks * 2 * sizeof(T)), mean_bytes = pad(size_t(p.rows) * 2 * sizeof(T));
+    const size_t col_bytes = cols ? size_t(groups) * 2 * p.n * sizeof(T) : 0;
+    NkWorkspace ws(ctx);
+    int st = ws.get(part_bytes + mean_bytes + col_bytes);
+    if (st) return st;
+    T *part = static_cast<T*>(ws.ptr), *means = reinterpret_cast<T*>(static_cast<char*>(ws.ptr) + part_bytes);
+    T* col = cols ? reinterpret_cast<T*>(static_cast<char*>(ws.ptr) + part_bytes + mean_bytes) : nullptr;
+    if (a.out) {
+        nk_norm_chunk_sums_kernel<T, W><<<nk_grid_for(ctx, p.rows * chunks, 1, 32), NORM_THREADS, 0, ctx->stream>>>(a.err, a.src, a.gain, a.stats, part, p, chunks);
+        if ((st = nk_after_launch(ctx, "nk_norm_chunk_sums_kernel"))) return st;
+        nk_norm_row_means_kernel<T><<<nk_grid_for(ctx, p.rows, NORM_THREADS / 32, 8), NORM_THREADS, 0, ctx->stream>>>(part, means, p.rows, chunks, T(p.n));
+        if ((st = nk_after_launch(ctx, "nk_norm_row_means_kernel"))) return st;
+    }
+    nk_norm_columns_kernel<T, W><<<nk_grid_for(ctx, blocks_c * groups, 1, 32), NORM_THREADS, 0, ctx->stream>>>(a.out, a.err, a.src, a.gain, a.stats, means, col, p, groups, per);
+    if ((st = nk_after_launch(ctx, "nk_norm_columns_kernel")) || !cols) return st;
+    nk_norm_columns_finish_kernel<T><<<nk_grid_for(ctx, p.n, NORM_THREADS, 8), NORM_THREADS, 0, ctx->stream>>>(a.dgain, a.dgain_s, a.dshift, a.dshift_s, col, p.n, groups);
+    return nk_after_launch(ctx, "nk_norm_columns_finish_kernel");
+}
+template <class T>
+int backward(nk_ctx* ctx, const NormGrad<T>& a, const NormPlan& p) {
+    if ((!a.out || norm_vec<T>(p, 0, a.out)) && norm_vec<T>(p, 1, a.src) && norm_vec<T>(p, 2, a.err)) return backward_w<T, norm_w<T>()>(ctx, a, p);
+    return backward_w<T, 1>(ctx, a, p);
+}
+
+// a view of rank 1 with n elements, or NULL
+int norm_vector(nk_ctx* ctx, const char* who, nk_buf* buf, const int32_t* cfg, int32_t dtype, int64_t n, bool drain, void** ptr, int64_t* stride) {
+    *ptr = nullptr;
+    *stride = 1;
+    if (!buf) return NK_OK;
+    NkView v;
+    int st;
+    if ((st = nk_view_parse(ctx, who, buf, cfg, 1, dtype, &v))) return st;
+    if (drain && (st = nk_check_drain(ctx, who, v))) return st;
+    if (v.size != n) return nk_fail(ctx, NK_ERR_BAD_ARG, "%s: %lld elements, rows have %lld", who, (long long)v.size, (long long)n);
+    *ptr = static_cast<char*>(buf->ptr) + v.base * int64_t(nk_dtype_size(dtype));
+    *stride = v.estride[0];
+    return NK_OK;
+}
+int norm_stats(nk_ctx* ctx, const char* who, const nk_buf* stats, int32_t dtype, int64_t rows) {
+    if (stats->magic != 0x4e4b4246) return nk_fail(ctx, NK_ERR_BAD_ARG, "%s: invalid handle of the statistics' buffer", who);
+    if (stats->dtype != dtype || stats->device != ctx->device) return nk_fail(ctx, NK_ERR_BAD_ARG, "%s: the statistics' buffer is of another type or device", who);
+    if (stats->n_elems / 2 < rows) return nk_fail(ctx, NK_ERR_BOUNDS, "%s: the statistics need 2 * %lld elements, the buffer holds %lld", who, (long long)rows, (long long)stats->n_elems);
+    return NK_OK;
+}
+int norm_same_shape(nk_ctx* ctx, const char* who, const NkView& a, const NkView& b) {
+    for (int k = 0; k < a.rank; k++)
+        if (a.shape[k] != b.shape[k]) return nk_fail(ctx, NK_ERR_BAD_ARG, "%s: shapes differ at dim %d (%lld vs %lld)", who, k, (long long)a.shape[k], (long long)b.shape[k]);
+    return NK_OK;
+}
+
+template <class T> T* at(nk_buf* b, const NkView& v) { return static_cast<T*>(b->ptr) + v.base; }
+
+}  // namespace
+
+extern "C" int nk_layer_norm(nk_ctx* ctx, int32_t dtype, int32_t rank, nk_buf* drn, const int32_t* cfg0, nk_buf* src, const int32_t* cfg1, nk_buf* gain,
+                             const int32_t* cfg_gain, nk_buf* shift, const int32_t* cfg_shift, double eps, nk_buf* stats) {
+    NK_CHECK_CTX(ctx);
+    if (dtype != NK_F32 && dtype != NK_F64) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_layer_norm: dtype %d not supported (F32/F64 only)", dtype);
+    if (!(eps >= 0.0)) return nk_fail(ctx, NK_ERR_BAD_ARG, "nk_layer_norm: eps %g is not >= 0", eps);
+    NkView v0, v1;
+    int st;
+    if ((st = nk_view_parse(ctx, "nk_layer_norm(drain)", drn, cfg0, rank, dtype, &v0))) return st;
+    if ((st = nk_check_drain(ctx, "nk_layer_norm", v0))) return st;
+    if ((st = nk_view_parse(ctx, "nk_layer_norm(src)", src, cfg1, rank, dtype, &v1))) return st;
+    if ((st = norm_same_shape(ctx, "nk_layer_norm", v0, v1))) return st;
+    const NkView* views[3] = {&v0, &v1, nullptr};
+    NormPlan p;
+    norm_plan(views, &p);
+    void *g, *s;
+    if ((st = norm_vector(ctx, "nk_layer_norm(gain)", gain, cfg_gain, dtype, p.n, false, &g, &p.gain_s))) return st;
+    if ((st = norm_vector(ctx, "nk_layer_norm(shift)", shift, cfg_shift, dtype, p.n, false, &s, &p.shift_s))) return st;
+    if (stats && (st = norm_stats(ctx, "nk_layer_norm", stats, dtype, p.rows))) return st;
+    void* keep = stats ? stats->ptr : nullptr;
+    if (dtype == NK_F32) return forward<float>(ctx, at<float>(drn, v0), at<float>(src, v1), (float*)g, (float*)s, (float*)keep, p, eps);
+    return forward<double>(ctx, at<double>(drn, v0), at<double>(src, v1), (double*)g, (double*)s, (double*)keep, p, eps);
+}
+
+namespace {
+template <class T>
+int norm_grad(nk_ctx* ctx, nk_buf* dsrc, const NkView& v0, void* dgain, int64_t dgain_s, void* dshift, int64_t dshift_s, nk_buf* err, const NkView& v2, nk_buf* src,
+              const NkView& v1, void* gain, nk_buf* stats, const NormPlan& p) {
+    NormGrad<T> a;
+    a.out = dsrc ? at<T>(dsrc, v0) : nullptr;
+    a.dgain = static_cast<T*>(dgain); a.dgain_s = dgain_s;
+    a.dshift = static_cast<T*>(dshift); a.dshift_s = dshift_s;
+    a.err = at<T>(err, v2);
+    a.src = at<T>(src, v1);
+    a.gain = static_cast<const T*>(gain);
+    a.stats = static_cast<const T*>(stats->ptr);
+    return backward<T>(ctx, a, p);
+}
+}  // namespace
+
+extern "C" int nk_layer_norm_grad(nk_ctx* ctx, int32_t dtype, int32_t rank, nk_buf* dsrc, const int32_t* cfg_dsrc, nk_buf* dgain, const int32_t* cfg_dgain,
+                                  nk_buf* dshift, const int32_t* cfg_dshift, nk_buf* err, const int32_t* cfg_err, nk_buf* src, const int32_t* cfg1, nk_buf* gain,
+                                  const int32_t* cfg_gain, nk_buf* stats) {
+    NK_CHECK_CTX(ctx);
+    if (dtype != NK_F32 && dtype != NK_F64) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_layer_norm_grad: dtype %d not supported (F32/F64 only)", dtype);
+    if (!stats) return nk_fail(ctx, NK_ERR_BAD_ARG, "nk_layer_norm_grad: the forward call's statistics are needed");
+    NkView v0, v1, v2;
+    int st;
+    if ((st = nk_view_parse(ctx, "nk_layer_norm_grad(err)", err, cfg_err, rank, dtype, &v2))) return st;
+    if ((st = nk_view_parse(ctx, "nk_layer_norm_grad(src)", src, cfg1, rank, dtype, &v1))) return st;
+    if ((st = norm_same_shape(ctx, "nk_layer_norm_grad", v2, v1))) return st;
+    if (dsrc) {
+        if ((st = nk_view_parse(ctx, "nk_layer_norm_grad(dsrc)", dsrc, cfg_dsrc, rank, dtype, &v0))) return st;
+        if ((st = nk_check_drain(ctx, "nk_layer_norm_grad", v0))) return st;
+        if ((st = norm_same_shape(ctx, "nk_layer_norm_grad", v0, v1))) return st;
+    }
+    const NkView* views[3] = {dsrc ? &v0 : nullptr, &v1, &v2};
+    NormPlan p;
+    norm_plan(views, &p);
+    void *g, *dg, *ds;
+    int64_t dgain_s, dshift_s;
+    if ((st = norm_vector(ctx, "nk_layer_norm_grad(gain)", gain, cfg_gain, dtype, p.n, false, &g, &p.gain_s))) return st;
+    if ((st = norm_vector(ctx, "nk_layer_norm_grad(dgain)", dgain, cfg_dgain, dtype, p.n, true, &dg, &dgain_s))) return st;
+    if ((st = norm_vector(ctx, "nk_layer_norm_grad(dshift)", dshift, cfg_dshift, dtype, p.n, true, &ds, &dshift_s))) return st;
+    if ((st = norm_stats(ctx, "nk_layer_norm_grad", stats, dtype, p.rows))) return st;
+    if (!dsrc && !dg && !ds) return NK_OK;
+    if (dtype == NK_F32) return norm_grad<float>(ctx, dsrc, v0, dg, dgain_s, ds, dshift_s, err, v2, src, v1, g, stats, p);
+    return norm_grad<double>(ctx, dsrc, v0, dg, dgain_s, ds, dshift_s, err, v2, src, v1, g, stats, p);
+}

@@ -307,6 +307,74 @@ def run_matmul(a: Tensor, b: Tensor) -> Tensor:
     return out
 
 
+def _vector_of(t: Optional[Tensor], x: Tensor, what: str) -> None:
+    if t is None:
+        return
+    if t.shape[-1] != x.shape[-1] or t.size != x.shape[-1]:
+        raise ValueError(f"{what} of shape {t.shape} does not fit rows of {x.shape[-1]} elements")
+
+
+def run_layer_norm(x: Tensor, gain: Optional[Tensor], shift: Optional[Tensor], eps: float, keep: bool) -> Tuple[Tensor, Optional[Tensor]]:
+    """Operation "layerNorm" over the last axis; with `keep` also the rows' statistics that the backward pass reads."""
+    _vector_of(gain, x, "the gain")
+    _vector_of(shift, x, "the shift")
+    operands = [t for t in (x, gain, shift) if t is not None]
+    dev = _common_device(operands)
+    out = _new_output(x.dtype, x.shape, dev)
+    stats = _new_output(x.dtype, (2, x.size // x.shape[-1]), dev) if keep else None
+    call = ExecutionCall([out] + operands + ([stats] if keep else []), "layerNorm", dev, -1, {"gain": gain, "shift": shift, "stats": stats, "eps": float(eps)})
+    return _execute_on_common_device(call, B.backend().implementation_for("layerNorm", B.LAYER_NORM)), stats
+
+
+def run_layer_norm_gradients(err: Tensor, x: Tensor, gain: Optional[Tensor], shift: Optional[Tensor], stats: Tensor, wanted: Sequence[bool]) -> List[Optional[Tensor]]:
+    """The errors of x, gain and shift (None where not wanted), from one call."""
+    dev = stats.device
+    drains = [_new_output(t.dtype, t.shape, dev) if w else None for t, w in zip((x, gain, shift), wanted)]
+    operands = [err, x, stats] + ([gain] if gain is not None else []) + [d for d in drains if d is not None]
+    call = ExecutionCall(operands, "layerNorm", dev, 0, {"dsrc": drains[0], "dgain": drains[1], "dshift": drains[2], "gain": gain, "stats": stats})
+    _execute_on_common_device(call, B.CudaLayerNormGradients())
+    return drains
+
+
+def run_dropout(x: Tensor, p: float, seed: int, stream: int, residual: Optional[Tensor] = None) -> Tensor:
+    """Operation "dropout": the kept elements of x times 1 / (1 - p), the others 0; plus the residual."""
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual of shape {residual.shape} does not fit a tensor of shape {x.shape}")
+    for name, v in (("seed", seed), ("stream", stream)):
+        if not -(1 << 63) <= v < 1 << 63:
+            raise ValueError(f"{name} {v} does not fit 64 bits")
+    operands = [x] if residual is None else [x, residual]
+    dev = _common_device(operands)
+    out = _new_output(x.dtype, x.shape, dev)
+    call = ExecutionCall([out] + operands, "dropout", dev, -1, {"p": float(p), "seed": int(seed), "stream": int(stream)})
+    return _execute_on_common_device(call, B.backend().implementation_for("dropout", B.DROPOUT))
+
+
+def run_gated(x: Tensor, w_gate: Tensor, w_up: Tensor, fun: str, keep: bool) -> Tuple[Tensor, Optional[Tensor]]:
+    """Operation "gated": fun(x @ w_gate) * (x @ w_up); with `keep` also the two products that the backward pass reads."""
+    if fun not in L.GATES:
+        raise ValueError(f"'{fun}' is no gate; one of {', '.join(L.GATES)}")
+    if x.rank != 2 or w_gate.rank != 2 or w_up.rank != 2:
+        raise ValueError("the gated block needs three rank-2 tensors")
+    if w_gate.shape != w_up.shape or x.shape[1] != w_gate.shape[0]:
+        raise ValueError(f"shapes {x.shape}, {w_gate.shape} and {w_up.shape} do not make a gated block")
+    dev = _common_device([x, w_gate, w_up])
+    out = _new_output(x.dtype, (x.shape[0], w_gate.shape[1]), dev)
+    kept = _new_output(x.dtype, (2,) + out.shape, dev) if keep else None
+    call = ExecutionCall([out, x, w_gate, w_up] + ([kept] if keep else []), "gated", dev, -1, {"fun": fun})
+    return _execute_on_common_device(call, B.backend().implementation_for("gated", B.GATED)), kept
+
+
+def run_gated_gradients(err: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, kept: Tensor, fun: str, wanted: Sequence[bool]) -> List[Optional[Tensor]]:
+    """The errors of x and of both weights (None where not wanted), from one call."""
+    dev = kept.device
+    drains = [_new_output(t.dtype, t.shape, dev) if w else None for t, w in zip((x, w_gate, w_up), wanted)]
+    call = ExecutionCall([err, x, w_gate, w_up, kept] + [d for d in drains if d is not None], "gated", dev, 0,
+                         {"fun": fun, "dsrc": drains[0], "dgate": drains[1], "dup": drains[2]})
+    _execute_on_common_device(call, B.CudaGatedGradients())
+    return drains
+
+
 def choose_algorithm(a: Tensor, b: Tensor) -> str:
     if b.size == 1 or b.is_virtual:
         return B.BI_SCALAR_BROADCAST

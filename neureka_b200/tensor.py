@@ -280,6 +280,25 @@ class Tensor:
         from . import autograd
         return autograd.extreme(self, True)
 
+    def layer_norm(self, gain=None, shift=None, eps: float = 1e-5):
+        """Every row (the last axis) less its mean, over the square root of its variance + eps, times gain, plus shift. gain and shift are
+        vectors of the row's length (or None); differentiable in all three. (No counterpart in the reference.)"""
+        from . import autograd
+        return autograd.layer_norm(self, gain, shift, eps)
+
+    def dropout(self, p: float, seed: int, stream: int = 0, residual=None):
+        """The elements times 1 / (1 - p), each dropped (0) with probability p, 0 <= p < 1; plus the residual where one is given. Which
+        ones are dropped is a function of seed, stream and the element's row-major index: a training step gives each of its
+        calls another stream, and the same call drops the same elements again. Differentiable in both tensors. (No counterpart in the reference.)"""
+        from . import autograd
+        return autograd.dropout(self, p, seed, stream, residual)
+
+    def gated(self, w_gate, w_up, fun: str = "silu"):
+        """fun(self @ w_gate) * (self @ w_up), the first half of a gated feed-forward block, as one operation; fun is one of sig, silu, gelu,
+        relu, tanh, idy. Differentiable in all three. (No counterpart in the reference.)"""
+        from . import autograd
+        return autograd.gated(self, w_gate, w_up, fun)
+
     def backward(self, error=None):
         from . import autograd
         autograd.backward(self, error)

@@ -1,0 +1,103 @@
+"""Layer norm, dropout and the gated block without a GPU: the plain implementations that the GPU tests compare with, and what is refused
+before any device is needed."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import sublayer as S
+
+
+def test_generator_gives_the_published_words():
+    """The known answers of Philox4x32-10: counter and key all zeros, all ones, and digits of pi."""
+    def words(counter, key):
+        return [int(w) for w in S.philox4x32(counter, key)]
+    assert words([0, 0, 0, 0], (0, 0)) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    assert words([0xFFFFFFFF] * 4, (0xFFFFFFFF, 0xFFFFFFFF)) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    assert words([0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344], (0xA4093822, 0x299F31D0)) == [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+
+
+@pytest.mark.parametrize("fun", ["sig", "silu", "gelu", "relu", "tanh", "idy"])
+def test_plain_gradients_against_differences(fun):
+    rng = np.random.default_rng(3)
+    x, wg, wu, e = (rng.standard_normal(s) for s in ((3, 4), (4, 5), (4, 5), (3, 5)))
+    grads = S.gated_gradients(x, wg, wu, e, fun)
+    for i, a in enumerate((x, wg, wu)):
+        for at in np.ndindex(a.shape):
+            keep, h = a[at], 1e-6
+            a[at] = keep + h
+            up = (S.gated(x, wg, wu, fun)[0][0] * e).sum()
+            a[at] = keep - h
+            down = (S.gated(x, wg, wu, fun)[0][0] * e).sum()
+            a[at] = keep
+            assert abs((up - down) / (2 * h) - grads[i][0][at]) < 1e-7 * max(1, abs(grads[i][0][at]))
+
+
+def test_plain_norm_gradients_against_differences():
+    rng = np.random.default_rng(4)
+    x, gain, shift, e = rng.standard_normal((3, 7)), rng.standard_normal(7), rng.standard_normal(7), rng.standard_normal((3, 7))
+    grads = S.norm_gradients(x, gain, e, 1e-5, S.unit(np.float64))
+    for i, a in enumerate((x, gain, shift)):
+        for at in np.ndindex(a.shape):
+            keep, h = a[at], 1e-6
+            a[at] = keep + h
+            up = (S.norm(x, gain, shift, 1e-5)[0] * e).sum()
+            a[at] = keep - h
+            down = (S.norm(x, gain, shift, 1e-5)[0] * e).sum()
+            a[at] = keep
+            assert abs((up - down) / (2 * h) - grads[i][0][at]) < 1e-7 * max(1, abs(grads[i][0][at]))
+
+
+def test_refused_before_a_device_is_needed():
+    from neureka_b200 import _lib as L
+    from neureka_b200.tensor import Tensor
+    x, v = Tensor.of(np.float32, [4, 6], np.zeros(24)), Tensor.of(np.float32, [5], np.zeros(5))
+    w, w2 = Tensor.of(np.float32, [6, 3], np.zeros(18)), Tensor.of(np.float32, [6, 2], np.zeros(12))
+    with pytest.raises(ValueError, match="does not fit rows of 6"):
+        x.layer_norm(v)
+    with pytest.raises(ValueError, match="does not fit rows of 6"):
+        x.layer_norm(None, Tensor.of(np.float32, [4, 6], np.zeros(24)))
+    with pytest.raises(ValueError, match="residual"):
+        x.dropout(0.5, 1, 0, v)
+    with pytest.raises(ValueError, match="64 bits"):
+        x.dropout(0.5, 1 << 63)
+    with pytest.raises(ValueError, match="no gate"):
+        x.gated(w, w, "softplus")
+    with pytest.raises(ValueError, match="do not make"):
+        x.gated(w, w2)
+    with pytest.raises(ValueError, match="rank-2"):
+        x.gated(w, v)
+    for call in (lambda: x.layer_norm(), lambda: x.dropout(0.5, 1), lambda: x.gated(w, w)):
+        with pytest.raises(L.NeurekaCudaError, match="no CPU execution"):
+            call()
+
+
+def test_entry_points_refuse_a_missing_context():
+    from neureka_b200 import _lib as L
+    none = [None, None]
+    assert L.lib.nk_layer_norm(None, L.NK_F32, 2, *none * 4, 1e-5, None) == L.NK_ERR_BAD_ARG
+    assert L.lib.nk_layer_norm_grad(None, L.NK_F32, 2, *none * 6, None) == L.NK_ERR_BAD_ARG
+    assert L.lib.nk_dropout(None, L.NK_F32, 2, *none * 3, 0.5, 0, 0) == L.NK_ERR_BAD_ARG
+    assert L.lib.nk_gated(None, L.FUN["silu"], L.NK_F32, *none * 4, None) == L.NK_ERR_BAD_ARG
+    assert L.lib.nk_gated_grad(None, L.FUN["silu"], L.NK_F32, *none * 7, None) == L.NK_ERR_BAD_ARG
+    assert b"invalid context" in L.lib.nk_last_error(None)
+
+
+def test_registered_beside_the_other_operations():
+    from neureka_b200 import backend as B
+    pairs = set(B.CudaBackend().pairs())
+    assert {("layerNorm", B.LAYER_NORM), ("dropout", B.DROPOUT), ("gated", B.GATED)} <= pairs
+
+
+def test_vectors_of_any_view_are_described_with_one_dim():
+    """A gain or shift may be a row of a matrix, a slice with a step, or turned: the descriptor of rank 1 names the same elements."""
+    from neureka_b200 import backend as B
+    from neureka_b200.ndconf import NDConfiguration as ND
+    from neureka_b200.tensor import Tensor
+    m = Tensor.of(np.float32, [4, 12], np.arange(48))
+    column = Tensor.of(np.float32, [12, 4], np.arange(48))
+    for t in (m[2:3, 1:12:2], m[0:1, 0:12], column[2:9, 3:4].permute(1, 0), Tensor.of(np.float32, [5], np.arange(5))):
+        arr, _ = B._cfg_vector(t)
+        assert len(arr) == 5
+        flat = ND((int(arr[0]),), (int(arr[1]),), (int(arr[2]),), (int(arr[4]),), (int(arr[3]),))
+        assert flat.element_offsets().tolist() == t.ndconf.element_offsets().tolist()
