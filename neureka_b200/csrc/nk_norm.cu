@@ -5,7 +5,11 @@
 //
 // Every sum is taken in the tensor's type over a fixed partition of the row (or column), so the result does not depend on scheduling; v
 // comes from the differences to a mean that is known before (no difference of large sums).
+#include <cooperative_groups.h>
+
 #include "nk_internal.h"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -21,6 +25,7 @@ struct NormPlan {
     int64_t ext[NK_MAX_RANK];
     int64_t s[3][NK_MAX_RANK], inner[3];     // 0: drain, 1: source, 2: error; strides of the outer dims and of the normalised one
     int64_t gain_s, shift_s;                 // strides of gain and shift
+    int gain_v, shift_v;                     // 16-byte loads of them are possible
 };
 
 template <int OP>
@@ -51,6 +56,16 @@ __device__ __forceinline__ void norm_store(T* row, int64_t c, int64_t inner, int
     else row[c * inner] = v[0];
 }
 
+// W elements of gain or shift (all of them exist)
+template <class T, int W>
+__device__ __forceinline__ void norm_vector_load(const T* a, int64_t c, int64_t stride, int vec, T (&v)[W]) {
+    if (W > 1 && vec) *reinterpret_cast<typename NormVec<T, W>::type*>(v) = __ldg(reinterpret_cast<const typename NormVec<T, W>::type*>(a + c));
+    else {
+#pragma unroll
+        for (int j = 0; j < W; j++) v[j] = __ldg(a + (c + j) * stride);
+    }
+}
+
 constexpr int NORM_THREADS = 256;
 // sum over the CTA, the same value in every thread
 template <class T>
@@ -65,6 +80,275 @@ __device__ __forceinline__ T norm_cta_sum(T v, T* smem) {
 #pragma unroll
     for (int w = 1; w < NORM_THREADS / 32; w++) v += smem[w];
     return v;
+}
+
+// sum over a CTA of THREADS threads, the same value in every thread; smem is not in use when the call begins and may be used again after the next
+// barrier that follows the call
+template <class T, int THREADS>
+__device__ __forceinline__ T norm_sum(T v, T* smem) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = smem[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 32; w++) v += smem[w];
+    return v;
+}
+template <class T, int THREADS>
+__device__ __forceinline__ void norm_sum2(T& a, T& b, T (*smem)[THREADS / 32]) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+    if ((threadIdx.x & 31) == 0) { smem[0][threadIdx.x >> 5] = a; smem[1][threadIdx.x >> 5] = b; }
+    __syncthreads();
+    a = smem[0][0];
+    b = smem[1][0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 32; w++) { a += smem[0][w]; b += smem[1][w]; }
+}
+// (x - mean) * rstd * gain + shift for the vectors at c0 + (k * lanes + lane) * W, stored
+template <class T, int W, int NV>
+__device__ __forceinline__ void norm_results(T* y, const T* gain, const T* shift, const NormPlan& p, int64_t c0, int lane, int lanes, T mean, T rstd, T (&v)[NV][W]) {
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int64_t c = c0 + (k * lanes + lane) * W;
+        if (c >= p.n) continue;
+        T g[W], s[W];
+        if (gain) norm_vector_load<T, W>(gain, c, p.gain_s, p.gain_v, g);
+        if (shift) norm_vector_load<T, W>(shift, c, p.shift_s, p.shift_v, s);
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            v[k][j] = (v[k][j] - mean) * rstd;
+            if (gain) v[k][j] *= g[j];
+            if (shift) v[k][j] += s[j];
+        }
+        norm_store<T, W>(y, c, p.inner[0], p.n, v[k]);
+    }
+}
+
+// ---- rows that a group of lanes, a CTA or a cluster holds in registers ---------------------------------------------------------------
+// One pass over the data: x stays in registers between the mean, the variance and the result.
+
+// A row per group of G lanes, E elements per lane.
+template <class T, int W, int G, int E>
+__global__ void __launch_bounds__(256) nk_norm_lanes_kernel(T* out, const T* src, const T* __restrict__ gain, const T* __restrict__ shift, T* __restrict__ stats,
+                                                            const NormPlan p, T eps) {
+    constexpr int NV = E / W;
+    const int lane = threadIdx.x % G;
+    const int64_t rows_per = 256 / G;
+    const T n = T(p.n);
+    for (int64_t first = int64_t(blockIdx.x) * rows_per; first < p.rows; first += int64_t(gridDim.x) * rows_per) {
+        const int64_t row = first + threadIdx.x / G;
+        const bool mine = row < p.rows;
+        const int64_t r = mine ? row : p.rows - 1;
+        const T* x = src + norm_row<1>(p, r);
+        T v[NV][W], sum = T(0);
+#pragma unroll
+        for (int k = 0; k < NV; k++) norm_load<T, W>(x, (k * G + lane) * W, p.inner[1], p.n, v[k]);
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int j = 0; j < W; j++) sum += v[k][j];
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const T mean = sum / n;
+        T m2 = T(0);
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int j = 0; j < W; j++)
+                if ((k * G + lane) * W + j < p.n) m2 += (v[k][j] - mean) * (v[k][j] - mean);
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
+        const T rstd = T(1) / sqrt(m2 / n + eps);
+        if (!mine) continue;
+        if (stats && lane == 0) { stats[row] = mean; stats[p.rows + row] = rstd; }
+        norm_results<T, W, NV>(out + norm_row<0>(p, row), gain, shift, p, int64_t(0), lane, G, mean, rstd, v);
+    }
+}
+// A row per CTA, or per cluster of CTAs (each a slice of the row; their sums meet through distributed shared memory).
+template <class T, int W, int THREADS, int E>
+__global__ void __launch_bounds__(THREADS) nk_norm_cta_kernel(T* out, const T* src, const T* __restrict__ gain, const T* __restrict__ shift, T* __restrict__ stats,
+                                                              const NormPlan p, T eps) {
+    constexpr int NV = E / W;
+    __shared__ T warps[2][THREADS / 32], parts[2][2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int size = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+    const int64_t c0 = int64_t(rank) * THREADS * E, step = gridDim.x / unsigned(size);
+    const T n = T(p.n);
+    int turn = 0;
+    auto total = [&](T v, int which) {
+        v = norm_sum<T, THREADS>(v, warps[which]);
+        if (size == 1) return v;
+        if (threadIdx.x == 0) parts[turn & 1][which] = v;   // two rows' worth: a slow neighbour may still read the last row's
+        cluster.sync();
+        v = T(0);
+        for (int r = 0; r < size; r++) v += *cluster.map_shared_rank(&parts[turn & 1][which], r);
+        return v;
+    };
+    for (int64_t row = blockIdx.x / unsigned(size); row < p.rows; row += step, turn++) {
+        const T* x = src + norm_row<1>(p, row);
+        T v[NV][W], sum = T(0);
+#pragma unroll
+        for (int k = 0; k < NV; k++) norm_load<T, W>(x, c0 + (k * THREADS + int(threadIdx.x)) * W, p.inner[1], p.n, v[k]);
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int j = 0; j < W; j++) sum += v[k][j];
+        const T mean = total(sum, 0) / n;
+        T m2 = T(0);
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int j = 0; j < W; j++)
+                if (c0 + (k * THREADS + int(threadIdx.x)) * W + j < p.n) m2 += (v[k][j] - mean) * (v[k][j] - mean);
+        const T rstd = T(1) / sqrt(total(m2, 1) / n + eps);
+        if (stats && rank == 0 && threadIdx.x == 0) { stats[row] = mean; stats[p.rows + row] = rstd; }
+        norm_results<T, W, NV>(out + norm_row<0>(p, row), gain, shift, p, c0, threadIdx.x, THREADS, mean, rstd, v);
+    }
+    if (size > 1) cluster.sync();   // nobody leaves while its sums may still be read
+}
+
+// Backward, a row per step of a CTA (or cluster): a thread owns E columns and walks the rows blockIdx.x, blockIdx.x + grid, ...; its columns' sums
+// over these rows stay in registers and go to cols[(CTA * 2 + which) * n + column] at the end.
+template <class T, int W, int THREADS, int E>
+__global__ void __launch_bounds__(THREADS) nk_norm_grad_kernel(T* out, const T* err, const T* src, const T* __restrict__ gain, const T* __restrict__ stats, T* __restrict__ cols,
+                                                               const NormPlan p) {
+    constexpr int NV = E / W;
+    __shared__ T warps[2][2][THREADS / 32], parts[2][2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int size = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+    const int64_t c0 = int64_t(rank) * THREADS * E, step = gridDim.x / unsigned(size), first = blockIdx.x / unsigned(size);
+    const T n = T(p.n);
+    T gv[NV][W], sg[NV][W], ss[NV][W];
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            const int64_t c = c0 + (k * THREADS + int(threadIdx.x)) * W + j;
+            gv[k][j] = gain && c < p.n ? gain[c * p.gain_s] : T(1);
+            sg[k][j] = ss[k][j] = T(0);
+        }
+    int turn = 0;
+    for (int64_t row = first; row < p.rows; row += step, turn++) {
+        const T *x = src + norm_row<1>(p, row), *e = err + norm_row<2>(p, row);
+        const T mean = stats[row], rstd = stats[p.rows + row];
+        T xh[NV][W], ev[NV][W], s1 = T(0), s2 = T(0);
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int64_t c = c0 + (k * THREADS + int(threadIdx.x)) * W;
+            norm_load<T, W>(x, c, p.inner[1], p.n, xh[k]);
+            norm_load<T, W>(e, c, p.inner[2], p.n, ev[k]);   // zero past the end: nothing is added there
+        }
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                xh[k][j] = (xh[k][j] - mean) * rstd;
+                sg[k][j] += ev[k][j] * xh[k][j];
+                ss[k][j] += ev[k][j];
+                const T g = ev[k][j] * gv[k][j];
+                s1 += g;
+                s2 += g * xh[k][j];
+            }
+        if (!out) continue;
+        norm_sum2<T, THREADS>(s1, s2, warps[turn & 1]);
+        if (size > 1) {
+            if (threadIdx.x == 0) { parts[turn & 1][0] = s1; parts[turn & 1][1] = s2; }
+            cluster.sync();
+            s1 = s2 = T(0);
+            for (int r = 0; r < size; r++) {
+                const T* theirs = cluster.map_shared_rank(&parts[turn & 1][0], r);
+                s1 += theirs[0];
+                s2 += theirs[1];
+            }
+        }
+        const T m1 = s1 / n, m2 = s2 / n;
+        T* o = out + norm_row<0>(p, row);
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+#pragma unroll
+            for (int j = 0; j < W; j++) ev[k][j] = rstd * (ev[k][j] * gv[k][j] - m1 - xh[k][j] * m2);
+            norm_store<T, W>(o, c0 + (k * THREADS + int(threadIdx.x)) * W, p.inner[0], p.n, ev[k]);
+        }
+    }
+    if (size > 1) cluster.sync();   // nobody leaves while its sums may still be read
+    if (!cols) return;
+    T* part = cols + first * 2 * p.n;
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int64_t c = c0 + (k * THREADS + int(threadIdx.x)) * W;
+        norm_store<T, W>(part, c, 1, p.n, sg[k]);
+        norm_store<T, W>(part + p.n, c, 1, p.n, ss[k]);
+    }
+}
+// The same with a row per group of G lanes; the groups of a CTA add their column sums through shared memory at the end, in order.
+template <class T, int W, int G, int E>
+__global__ void __launch_bounds__(256) nk_norm_grad_lanes_kernel(T* out, const T* err, const T* src, const T* __restrict__ gain, const T* __restrict__ stats, T* __restrict__ cols,
+                                                                 const NormPlan p) {
+    constexpr int NV = E / W, ROWS = 256 / G;
+    __shared__ T sums[2][G * E];
+    const int lane = threadIdx.x % G, group = threadIdx.x / G;
+    const T n = T(p.n);
+    T gv[NV][W], sg[NV][W], ss[NV][W];
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            const int c = (k * G + lane) * W + j;
+            gv[k][j] = gain && c < p.n ? gain[c * p.gain_s] : T(1);
+            sg[k][j] = ss[k][j] = T(0);
+        }
+    for (int64_t base = int64_t(blockIdx.x) * ROWS; base < p.rows; base += int64_t(gridDim.x) * ROWS) {
+        const bool mine = base + group < p.rows;
+        const int64_t row = mine ? base + group : p.rows - 1;
+        const T *x = src + norm_row<1>(p, row), *e = err + norm_row<2>(p, row);
+        const T mean = stats[row], rstd = stats[p.rows + row];
+        T xh[NV][W], ev[NV][W], s1 = T(0), s2 = T(0);
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            norm_load<T, W>(x, (k * G + lane) * W, p.inner[1], p.n, xh[k]);
+            norm_load<T, W>(e, (k * G + lane) * W, p.inner[2], mine ? p.n : 0, ev[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                xh[k][j] = (xh[k][j] - mean) * rstd;
+                if (mine) sg[k][j] += ev[k][j] * xh[k][j];   // (the last row's values may not be finite)
+                ss[k][j] += ev[k][j];
+                const T g = ev[k][j] * gv[k][j];
+                s1 += g;
+                s2 += g * xh[k][j];
+            }
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) { s1 += __shfl_xor_sync(0xffffffffu, s1, o); s2 += __shfl_xor_sync(0xffffffffu, s2, o); }
+        if (!out || !mine) continue;
+        const T m1 = s1 / n, m2 = s2 / n;
+        T* o = out + norm_row<0>(p, row);
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+#pragma unroll
+            for (int j = 0; j < W; j++) ev[k][j] = rstd * (ev[k][j] * gv[k][j] - m1 - xh[k][j] * m2);
+            norm_store<T, W>(o, (k * G + lane) * W, p.inner[0], p.n, ev[k]);
+        }
+    }
+    if (!cols) return;
+    for (int r = 0; r < ROWS; r++) {
+        if (group == r) {
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    const int c = (k * G + lane) * W + j;
+                    sums[0][c] = r ? sums[0][c] + sg[k][j] : sg[k][j];
+                    sums[1][c] = r ? sums[1][c] + ss[k][j] : ss[k][j];
+                }
+        }
+        __syncthreads();
+    }
+    T* part = cols + int64_t(blockIdx.x) * 2 * p.n;
+    for (int64_t c = threadIdx.x; c < p.n; c += 256) { part[c] = sums[0][c]; part[p.n + c] = sums[1][c]; }
 }
 
 // ---- rows of any length: cut into chunks of NORM_THREADS * W * 8 elements, a CTA per chunk ---------------------------------------
@@ -209,15 +493,30 @@ __global__ void __launch_bounds__(NORM_THREADS) nk_norm_columns_kernel(T* out, c
         }
     }
 }
-// the groups' parts of the column sums, added in group order
+// The groups' parts of the column sums: 32 columns per CTA, eight threads per column take every eighth group, in order, and are added in order.
 template <class T>
 __global__ void __launch_bounds__(NORM_THREADS) nk_norm_columns_finish_kernel(T* dgain, int64_t dgain_s, T* dshift, int64_t dshift_s, const T* __restrict__ cols, int64_t n,
                                                                               int64_t groups) {
-    for (int64_t c = int64_t(blockIdx.x) * NORM_THREADS + threadIdx.x; c < n; c += int64_t(gridDim.x) * NORM_THREADS) {
+    __shared__ T sums[2][8][33];
+    const int lane = threadIdx.x & 31, slot = threadIdx.x >> 5;
+    for (int64_t c0 = int64_t(blockIdx.x) * 32; c0 < n; c0 += int64_t(gridDim.x) * 32) {
+        const int64_t c = c0 + lane;
         T sg = T(0), ss = T(0);
-        for (int64_t g = 0; g < groups; g++) { sg += cols[(g * 2) * n + c]; ss += cols[(g * 2 + 1) * n + c]; }
-        if (dgain) dgain[c * dgain_s] = sg;
-        if (dshift) dshift[c * dshift_s] = ss;
+        if (c < n) {
+#pragma unroll 8
+            for (int64_t g = slot; g < groups; g += 8) { sg += cols[(g * 2) * n + c]; ss += cols[(g * 2 + 1) * n + c]; }
+        }
+        __syncthreads();   // the sums of the columns before have been read
+        sums[0][slot][lane] = sg;
+        sums[1][slot][lane] = ss;
+        __syncthreads();
+        if (slot < 2 && c < n) {
+            T v = sums[slot][0][lane];
+#pragma unroll
+            for (int k = 1; k < 8; k++) v += sums[slot][k][lane];
+            if (slot == 0 && dgain) dgain[c * dgain_s] = v;
+            if (slot == 1 && dshift) dshift[c * dshift_s] = v;
+        }
     }
 }
 
@@ -251,8 +550,53 @@ bool norm_vec(const NormPlan& p, int t, const T* base) {
     return true;
 }
 
+// one resident wave at most; a cluster's CTAs lie side by side
+template <class... A>
+int norm_launch(nk_ctx* ctx, const char* name, void (*kern)(A...), int64_t rows, int threads, int cluster, int per_sm, A... args) {
+    int64_t units = int64_t(ctx->prop.multiProcessorCount) * per_sm / cluster;
+    if (units > rows) units = rows;
+    if (units < 1) units = 1;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(unsigned(units * cluster));
+    cfg.blockDim = dim3(threads);
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e != cudaSuccess) return nk_cuda_fail(ctx, e, name);
+    return nk_after_launch(ctx, name);
+}
+// elements that a thread of the CTA kernels holds at most, and the longest row that they take (a cluster of eight)
+template <class T> constexpr int norm_e() { return 128 / int(sizeof(T)); }
+
+template <class T, int W>
+int forward_rows(nk_ctx* ctx, T* out, const T* src, const T* gain, const T* shift, T* stats, const NormPlan& p, T eps) {
+    constexpr int E = norm_e<T>();
+#define NK_LANES(G, EL) return norm_launch(ctx, "nk_norm_lanes_kernel", nk_norm_lanes_kernel<T, W, G, EL>, (p.rows + 256 / G - 1) / (256 / G), 256, 1, 32, out, src, gain, shift, stats, p, eps)
+#define NK_CTA(TH, EL, C) return norm_launch(ctx, "nk_norm_cta_kernel", nk_norm_cta_kernel<T, W, TH, EL>, p.rows, TH, C, 16, out, src, gain, shift, stats, p, eps)
+    if (p.n <= 32) NK_LANES(8, 4);
+    if (p.n <= 128) NK_LANES(32, 4);
+    if (p.n <= 256) NK_LANES(32, 8);
+    if (p.n <= 512) NK_LANES(32, 16);
+    if (p.n <= 1024) NK_CTA(128, 8, 1);
+    if (p.n <= 2048) NK_CTA(256, 8, 1);
+    if (p.n <= 4096) NK_CTA(256, 16, 1);
+    if (p.n <= 256 * E) NK_CTA(256, E, 1);
+    if (p.n <= 512 * E) NK_CTA(512, E, 1);
+    const int cluster = p.n <= 1024 * E ? 2 : p.n <= 2048 * E ? 4 : 8;
+    NK_CTA(512, E, cluster);
+#undef NK_LANES
+#undef NK_CTA
+}
+
 template <class T, int W>
 int forward_w(nk_ctx* ctx, T* out, const T* src, const T* gain, const T* shift, T* stats, const NormPlan& p, T eps) {
+    if (p.n <= 4096 * norm_e<T>()) return forward_rows<T, W>(ctx, out, src, gain, shift, stats, p, eps);
     constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
     const int64_t chunks = (p.n + L - 1) / L;
     NkWorkspace ws(ctx);
@@ -277,8 +621,64 @@ struct NormGrad {
     const T *err, *src, *gain, *stats;
     int64_t dgain_s, dshift_s;
 };
+template <class T>
+int columns_finish(nk_ctx* ctx, const NormGrad<T>& a, const T* cols, int64_t n, int64_t groups) {
+    nk_norm_columns_finish_kernel<T><<<nk_grid_for(ctx, n, 32, 32), NORM_THREADS, 0, ctx->stream>>>(a.dgain, a.dgain_s, a.dshift, a.dshift_s, cols, n, groups);
+    return nk_after_launch(ctx, "nk_norm_columns_finish_kernel");
+}
+template <class T, int W>
+int backward_rows(nk_ctx* ctx, const NormGrad<T>& a, const NormPlan& p) {
+    constexpr int E = norm_e<T>() / 2;
+    const int64_t sms = ctx->prop.multiProcessorCount;
+    // Few rows per CTA cost column sums that go to memory and back, few CTAs latency: one resident wave, at least four rows each where there are many
+    const bool cols = a.dgain || a.dshift;
+    auto units = [&](int64_t rows, int per_sm, int cluster) {
+        int64_t u = sms * per_sm / cluster, most = (rows + 3) / 4 > sms / cluster ? (rows + 3) / 4 : sms / cluster;
+        if (u > most) u = most;
+        if (u > rows) u = rows;
+        return u < 1 ? 1 : u;
+    };
+    int64_t groups;
+    T* part = nullptr;
+    NkWorkspace ws(ctx);
+    int st;
+    auto space = [&]() {
+        if (!cols) return int(NK_OK);
+        const int s = ws.get(size_t(groups) * 2 * p.n * sizeof(T));
+        part = static_cast<T*>(ws.ptr);
+        return s;
+    };
+#define NK_LANES(G, EL, PER)                                                                                                                                       \
+    do {                                                                                                                                                           \
+        groups = units((p.rows + 256 / G - 1) / (256 / G), PER, 1);                                                                                                \
+        if ((st = space())) return st;                                                                                                                             \
+        st = norm_launch(ctx, "nk_norm_grad_lanes_kernel", nk_norm_grad_lanes_kernel<T, W, G, EL>, groups, 256, 1, PER, a.out, a.err, a.src, a.gain, a.stats, part, p); \
+    } while (0)
+#define NK_CTA(TH, EL, C, PER)                                                                                                                                     \
+    do {                                                                                                                                                           \
+        groups = units(p.rows, PER, C);                                                                                                                            \
+        if ((st = space())) return st;                                                                                                                             \
+        st = norm_launch(ctx, "nk_norm_grad_kernel", nk_norm_grad_kernel<T, W, TH, EL>, groups, TH, C, PER, a.out, a.err, a.src, a.gain, a.stats, part, p);              \
+    } while (0)
+    if (p.n <= 32) NK_LANES(8, 4, 4);
+    else if (p.n <= 128) NK_LANES(32, 4, 4);
+    else if (p.n <= 256) NK_LANES(32, 8, 4);
+    else if (p.n <= 1024) NK_CTA(128, 8, 1, 6);
+    else if (p.n <= 2048) NK_CTA(256, 8, 1, 3);
+    else if (p.n <= 256 * E) NK_CTA(256, E, 1, 2);
+    else if (p.n <= 512 * E) NK_CTA(512, E, 1, 1);
+    else if (p.n <= 1024 * E) NK_CTA(512, E, 2, 1);
+    else if (p.n <= 2048 * E) NK_CTA(512, E, 4, 1);
+    else NK_CTA(512, E, 8, 1);
+#undef NK_LANES
+#undef NK_CTA
+    if (st || !cols) return st;
+    return columns_finish(ctx, a, static_cast<const T*>(part), p.n, groups);
+}
+
 template <class T, int W>
 int backward_w(nk_ctx* ctx, const NormGrad<T>& a, const NormPlan& p) {
+    if (p.n <= 2048 * norm_e<T>()) return backward_rows<T, W>(ctx, a, p);
     constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
     const int64_t chunks = (p.n + L - 1) / L, blocks_c = (p.n + NORM_THREADS * W - 1) / (NORM_THREADS * W);
     const bool cols = a.dgain || a.dshift;
@@ -303,8 +703,7 @@ int backward_w(nk_ctx* ctx, const NormGrad<T>& a, const NormPlan& p) {
     }
     nk_norm_columns_kernel<T, W><<<nk_grid_for(ctx, blocks_c * groups, 1, 32), NORM_THREADS, 0, ctx->stream>>>(a.out, a.err, a.src, a.gain, a.stats, means, col, p, groups, per);
     if ((st = nk_after_launch(ctx, "nk_norm_columns_kernel")) || !cols) return st;
-    nk_norm_columns_finish_kernel<T><<<nk_grid_for(ctx, p.n, NORM_THREADS, 8), NORM_THREADS, 0, ctx->stream>>>(a.dgain, a.dgain_s, a.dshift, a.dshift_s, col, p.n, groups);
-    return nk_after_launch(ctx, "nk_norm_columns_finish_kernel");
+    return columns_finish(ctx, a, static_cast<const T*>(col), p.n, groups);
 }
 template <class T>
 int backward(nk_ctx* ctx, const NormGrad<T>& a, const NormPlan& p) {
@@ -360,6 +759,8 @@ extern "C" int nk_layer_norm(nk_ctx* ctx, int32_t dtype, int32_t rank, nk_buf* d
     if ((st = norm_vector(ctx, "nk_layer_norm(gain)", gain, cfg_gain, dtype, p.n, false, &g, &p.gain_s))) return st;
     if ((st = norm_vector(ctx, "nk_layer_norm(shift)", shift, cfg_shift, dtype, p.n, false, &s, &p.shift_s))) return st;
     if (stats && (st = norm_stats(ctx, "nk_layer_norm", stats, dtype, p.rows))) return st;
+    p.gain_v = p.gain_s == 1 && reinterpret_cast<uintptr_t>(g) % 16 == 0;
+    p.shift_v = p.shift_s == 1 && reinterpret_cast<uintptr_t>(s) % 16 == 0;
     void* keep = stats ? stats->ptr : nullptr;
     if (dtype == NK_F32) return forward<float>(ctx, at<float>(drn, v0), at<float>(src, v1), (float*)g, (float*)s, (float*)keep, p, eps);
     return forward<double>(ctx, at<double>(drn, v0), at<double>(src, v1), (double*)g, (double*)s, (double*)keep, p, eps);
