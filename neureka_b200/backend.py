@@ -71,16 +71,17 @@ class ExecutionCall:
 
 
 def _cfg(t: Tensor):
-    arr = t.ndconf.as_inline_array()
-    return arr, arr.ctypes.data_as(C.POINTER(C.c_int32))
+    """The configuration (which has to outlive the call) and its descriptor for the library."""
+    c = t.ndconf
+    return c, c.inline_pointer
 
 
 def _cfg_virtual(t: Tensor):
     """_cfg for an operand that may stay virtual: every index maps to its one element."""
     if not t.is_virtual:
         return _cfg(t)
-    arr = NDConfiguration.virtual_of(t.shape).as_inline_array()
-    return arr, arr.ctypes.data_as(C.POINTER(C.c_int32))
+    c = NDConfiguration.virtual_of(t.shape)
+    return c, c.inline_pointer
 
 
 def _same_type(call: ExecutionCall, n: int) -> int:
@@ -279,12 +280,12 @@ def _cfg_vector(t: Tensor):
     if c.rank == 1:
         return _cfg(t)
     base = sum(o * s for o, s in zip(c.offset, c.strides))
-    arr = np.array((c.shape[-1], 1, 1, base, c.strides[-1] * c.spread[-1]), dtype=np.int32)
-    return arr, arr.ctypes.data_as(C.POINTER(C.c_int32))
+    v = NDConfiguration(c.shape[-1:], (1,), (1,), (c.strides[-1] * c.spread[-1],), (base,))
+    return v, v.inline_pointer
 
 
 def _buf_cfg(t: Optional[Tensor], cfg=_cfg):
-    """An operand as the C ABI takes it -- buffer, descriptor, and the array that backs the descriptor -- or nothing at all."""
+    """An operand as the C ABI takes it -- buffer, descriptor, and the configuration that backs the descriptor -- or nothing at all."""
     if t is None:
         return None, None, None
     keep, c = cfg(t)

@@ -267,7 +267,8 @@ class CudaDevice:
         return self
 
     def has(self, tensor) -> bool:
-        return tensor in self._stored and isinstance(tensor._data, CudaData) and tensor._data.device is self
+        data = tensor._data
+        return isinstance(data, CudaData) and data.device is self and tensor in self._stored
 
     contains = has
 

@@ -7,8 +7,10 @@ A view of a flat data array = five int vectors of length rank: shape, strides, i
 """
 from __future__ import annotations
 
+import ctypes as C
 from dataclasses import dataclass
 from enum import Enum
+from functools import cached_property, lru_cache
 from typing import Sequence, Tuple
 
 import numpy as np
@@ -70,25 +72,19 @@ class NDConfiguration:
     @staticmethod
     def of_shape(shape, layout: Layout = Layout.ROW_MAJOR) -> "NDConfiguration":
         """The configuration of a freshly created tensor (NDConstructor: row-major strides and indicesMap)."""
-        shape = tuple(int(x) for x in shape)
-        rm = Layout.ROW_MAJOR.new_strides_for(shape)
-        strides = layout.new_strides_for(shape) if layout is Layout.COLUMN_MAJOR else rm
-        n = len(shape)
-        return NDConfiguration.of(shape, strides, rm, (1,) * n, (0,) * n)
+        return _of_shape(tuple(int(x) for x in shape), layout)
 
     @staticmethod
     def virtual_of(shape) -> "NDConfiguration":
         """VirtualNDConfiguration (ndim/config/types/views/virtual/VirtualNDConfiguration.java): one element stands for all."""
-        shape = tuple(int(x) for x in shape)
-        z = (0,) * len(shape)
-        return NDConfiguration(shape, z, z, z, z, True)
+        return _virtual_of(tuple(int(x) for x in shape))
 
-    # ---- queries -----------------------------------------------------------------------------------
-    @property
+    # ---- queries (a configuration never changes: what is asked for with every call is worked out once) -----
+    @cached_property
     def rank(self) -> int:
         return len(self.shape)
 
-    @property
+    @cached_property
     def size(self) -> int:
         s = 1
         for d in self.shape:
@@ -98,6 +94,11 @@ class NDConfiguration:
     def as_inline_array(self) -> np.ndarray:
         """asInlineArray (NDConfiguration.java:335-345): [shape | strides | indicesMap | offset | spread]."""
         return np.array(self.shape + self.strides + self.indices_map + self.offset + self.spread, dtype=np.int32)
+
+    @cached_property
+    def inline_pointer(self):
+        """as_inline_array for a call of the library: a pointer to its ints, which live as long as the configuration."""
+        return self.as_inline_array().ctypes.data_as(C.POINTER(C.c_int32))
 
     def is_compact(self) -> bool:
         """isCompact (NDConfiguration.java:386-392)."""
@@ -181,3 +182,18 @@ class NDConfiguration:
         new_spread = tuple(1 if f < 0 else self.spread[f] for f in new_form)
         new_offset = tuple(0 if f < 0 else self.offset[f] for f in new_form)
         return NDConfiguration.of(new_shape, new_strides, new_imap, new_spread, new_offset)
+
+
+# A program makes tensors of the same few shapes over and over: their (immutable) configurations are shared.
+@lru_cache(maxsize=4096)
+def _of_shape(shape: Tuple[int, ...], layout: Layout) -> NDConfiguration:
+    rm = Layout.ROW_MAJOR.new_strides_for(shape)
+    strides = layout.new_strides_for(shape) if layout is Layout.COLUMN_MAJOR else rm
+    n = len(shape)
+    return NDConfiguration.of(shape, strides, rm, (1,) * n, (0,) * n)
+
+
+@lru_cache(maxsize=4096)
+def _virtual_of(shape: Tuple[int, ...]) -> NDConfiguration:
+    z = (0,) * len(shape)
+    return NDConfiguration(shape, z, z, z, z, True)

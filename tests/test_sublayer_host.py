@@ -97,7 +97,7 @@ def test_vectors_of_any_view_are_described_with_one_dim():
     m = Tensor.of(np.float32, [4, 12], np.arange(48))
     column = Tensor.of(np.float32, [12, 4], np.arange(48))
     for t in (m[2:3, 1:12:2], m[0:1, 0:12], column[2:9, 3:4].permute(1, 0), Tensor.of(np.float32, [5], np.arange(5))):
-        arr, _ = B._cfg_vector(t)
-        assert len(arr) == 5
-        flat = ND((int(arr[0]),), (int(arr[1]),), (int(arr[2]),), (int(arr[4]),), (int(arr[3]),))
+        _, at = B._cfg_vector(t)
+        shape, strides, indices_map, offset, spread = (at[i] for i in range(5))
+        flat = ND((shape,), (strides,), (indices_map,), (spread,), (offset,))
         assert flat.element_offsets().tolist() == t.ndconf.element_offsets().tolist()
