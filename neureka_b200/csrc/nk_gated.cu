@@ -1,25 +1,11 @@
 // The gated feed-forward block (no counterpart in the reference):
 //   g = x Wg, u = x Wu, y = f(g) * u;   dg = e * u * f'(g), du = e * f(g), dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du.
-// f and f' are the framework's own functions (nk_scalarfun.cuh, which wants -fmad=false; the products below say fma).
 //
 // nk_gated_tile_kernel: any sizes, any strides, both types. Both products of a tile share the panel of x and end in the same thread, so the
 // activation and the product with it happen in registers.
-#include "nk_gated.h"
-#include "nk_scalarfun.cuh"
+#include "nk_gated.cuh"
 
 namespace {
-
-template <class T>
-__device__ __forceinline__ T gate_fun(int f, bool derive, T x) {
-    switch (f) {
-        case NK_FUN_SIG: return nkf::fun(NK_FUN_SIG, derive, x);
-        case NK_FUN_SILU: return nkf::fun(NK_FUN_SILU, derive, x);
-        case NK_FUN_GELU: return nkf::fun(NK_FUN_GELU, derive, x);
-        case NK_FUN_RELU: return nkf::fun(NK_FUN_RELU, derive, x);
-        case NK_FUN_TANH: return nkf::fun(NK_FUN_TANH, derive, x);
-        default: return nkf::fun(NK_FUN_IDY, derive, x);
-    }
-}
 
 // ---- the tile kernel -------------------------------------------------------------------------------------------------------------
 // FORWARD: C_i = A_0 B_i, out_0 = f(C_0) * C_1 (C_i kept where wanted).  TWO: out_i = A_0 B_i.  SUM: out_0 = A_0 B_0 + A_1 B_1.
@@ -127,6 +113,11 @@ GatedMatrix turned(const GatedMatrix& m) { return GatedMatrix{m.ptr, m.cs, m.rs}
 
 template <class T>
 int forward(nk_ctx* ctx, const GatedCall& c) {
+    if (sizeof(T) == 4) {
+        bool handled = false;
+        const int st = nk_gated_tc_forward(ctx, c, &handled);
+        if (st || handled) return st;
+    }
     GatedTile p;
     memset(&p, 0, sizeof(p));
     p.fun = c.fun;
@@ -139,6 +130,11 @@ int forward(nk_ctx* ctx, const GatedCall& c) {
 }
 template <class T>
 int backward(nk_ctx* ctx, const GatedCall& c) {
+    if (sizeof(T) == 4) {
+        bool handled = false;
+        const int st = nk_gated_tc_backward(ctx, c, &handled);
+        if (st || handled) return st;
+    }
     NkWorkspace ws(ctx);
     int st = ws.get(size_t(c.T) * c.H * 2 * sizeof(T));
     if (st) return st;

@@ -1,0 +1,48 @@
+// The gated feed-forward block: what the kernel families behind nk_gated / nk_gated_grad share.
+// f and f' are the framework's own functions (nk_scalarfun.cuh: the units are compiled with -fmad=false, products say fma).
+#pragma once
+#include "nk_internal.h"
+#include "nk_scalarfun.cuh"
+
+// A matrix: element (r, c) at base[r * rs + c * cs].
+struct GatedMatrix {
+    void* ptr;      // null: not wanted
+    int64_t rs, cs;
+};
+
+// One call. T tokens, D features of the model, H hidden ones.
+struct GatedCall {
+    int fun;
+    int64_t T, D, H;
+    GatedMatrix x, w[2];      // [T, D]; gate and up [D, H]
+    GatedMatrix y;            // forward: [T, H]
+    void *gate, *up;          // x @ w[0], x @ w[1], row-major [T, H]; forward: null where nobody keeps them
+    GatedMatrix err;          // backward: [T, H]
+    GatedMatrix dx, dw[2];    // backward
+};
+
+template <class T>
+__device__ __forceinline__ T gate_fun(int f, bool derive, T x) {
+    switch (f) {
+        case NK_FUN_SIG: return nkf::fun(NK_FUN_SIG, derive, x);
+        case NK_FUN_SILU: return nkf::fun(NK_FUN_SILU, derive, x);
+        case NK_FUN_GELU: return nkf::fun(NK_FUN_GELU, derive, x);
+        case NK_FUN_RELU: return nkf::fun(NK_FUN_RELU, derive, x);
+        case NK_FUN_TANH: return nkf::fun(NK_FUN_TANH, derive, x);
+        default: return nkf::fun(NK_FUN_IDY, derive, x);
+    }
+}
+// CASE(FUN) for the function of a call
+#define NK_GATE_SWITCH(fun, CASE)                 \
+    switch (fun) {                                \
+        case NK_FUN_SIG: CASE(NK_FUN_SIG); break;   \
+        case NK_FUN_SILU: CASE(NK_FUN_SILU); break; \
+        case NK_FUN_GELU: CASE(NK_FUN_GELU); break; \
+        case NK_FUN_RELU: CASE(NK_FUN_RELU); break; \
+        case NK_FUN_TANH: CASE(NK_FUN_TANH); break; \
+        default: CASE(NK_FUN_IDY); break;           \
+    }
+
+// Many tokens in F32 on the tensor cores (nk_gated_tc.cu); *handled stays false where the call is not theirs.
+int nk_gated_tc_forward(nk_ctx* ctx, const GatedCall& c, bool* handled);
+int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled);
