@@ -113,6 +113,7 @@ GatedMatrix turned(const GatedMatrix& m) { return GatedMatrix{m.ptr, m.cs, m.rs}
 
 template <class T>
 int forward(nk_ctx* ctx, const GatedCall& c) {
+    if (nk_gated_few(c)) return nk_gated_few_forward<T>(ctx, c);
     if (sizeof(T) == 4) {
         bool handled = false;
         const int st = nk_gated_tc_forward(ctx, c, &handled);
@@ -141,6 +142,7 @@ int backward(nk_ctx* ctx, const GatedCall& c) {
     T *dg = static_cast<T*>(ws.ptr), *du = dg + c.T * c.H;
     nk_gated_errors_kernel<T><<<nk_grid_for(ctx, c.T * c.H, 256, 8), 256, 0, ctx->stream>>>(c, dg, du);
     if ((st = nk_after_launch(ctx, "nk_gated_errors_kernel"))) return st;
+    if (nk_gated_few(c)) return nk_gated_few_backward<T>(ctx, c, dg, du);
     const GatedMatrix mg{dg, c.H, 1}, mu{du, c.H, 1};
     GatedTile p;
     memset(&p, 0, sizeof(p));

@@ -46,3 +46,8 @@ __device__ __forceinline__ T gate_fun(int f, bool derive, T x) {
 // Many tokens in F32 on the tensor cores (nk_gated_tc.cu); *handled stays false where the call is not theirs.
 int nk_gated_tc_forward(nk_ctx* ctx, const GatedCall& c, bool* handled);
 int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled);
+
+// Few tokens, both types (nk_gated_few.cu). dg and du: row-major [T, H].
+bool nk_gated_few(const GatedCall& c);
+template <class T> int nk_gated_few_forward(nk_ctx* ctx, const GatedCall& c);
+template <class T> int nk_gated_few_backward(nk_ctx* ctx, const GatedCall& c, const T* dg, const T* du);
