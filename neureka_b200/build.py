@@ -50,6 +50,7 @@ SOURCES = [
     ("nk_gated.cu", ["-fmad=false"]),
     ("nk_gated_tc.cu", ["-fmad=false"]),
     ("nk_gated_few.cu", ["-fmad=false"]),
+    ("nk_gated_narrow.cu", ["-fmad=false"]),
     ("nk_probe.cu", []),
     ("nk_sum_static.cu", ["-fmad=false"]),
     ("nk_jrand.cpp", ["-Xcompiler", "-ffp-contract=off"]),

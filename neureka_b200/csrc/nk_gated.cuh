@@ -51,3 +51,10 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled);
 bool nk_gated_few(const GatedCall& c);
 template <class T> int nk_gated_few_forward(nk_ctx* ctx, const GatedCall& c);
 template <class T> int nk_gated_few_backward(nk_ctx* ctx, const GatedCall& c, const T* dg, const T* du);
+
+// Some tokens in F32 (nk_gated_narrow.cu). dx: hi and lo are panels [T][2 * nk_gated_narrow_columns(H)] of dg and du, zero past H; the tickets are zero.
+bool nk_gated_narrow(const nk_ctx* ctx, const GatedCall& c);
+int nk_gated_narrow_forward(nk_ctx* ctx, const GatedCall& c);
+int64_t nk_gated_narrow_columns(int64_t H);
+void nk_gated_narrow_dx_needs(nk_ctx* ctx, const GatedCall& c, size_t* part_bytes, int* tickets);
+int nk_gated_narrow_dx(nk_ctx* ctx, const GatedCall& c, const float* hi, const float* lo, float* parts, int* tickets);

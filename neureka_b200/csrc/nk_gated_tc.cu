@@ -80,11 +80,15 @@ struct ErrorPanels {
     float *t_hi[2], *t_lo[2];   // [H][Tp] of dg and of du; null: not wanted
     int64_t Hp, Tp;
     int err_vec, kept_vec;      // 16-byte loads along the rows
+    int* tickets;               // cleared
+    int n_tickets;
 };
 // 32 tokens x 128 hidden features per CTA: 12 bytes read and 32 written per element, four elements per thread and access.
 template <int FUN>
 __global__ void __launch_bounds__(256) nk_gated_errors_split_kernel(const GatedCall c, const ErrorPanels p, int64_t tiles_h) {
     __shared__ float tile[2][32][129];
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < p.n_tickets; i += 256) p.tickets[i] = 0;
     const int64_t t0 = (blockIdx.x / tiles_h) * 32, h0 = (blockIdx.x % tiles_h) * 128;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float *err = static_cast<const float*>(c.err.ptr), *gate = static_cast<const float*>(c.gate), *up = static_cast<const float*>(c.up);
@@ -182,7 +186,7 @@ int product(nk_ctx* ctx, const TcShape& shape, int64_t Kp, const TcPanels& a, co
 }
 // sizes that the tensor-core path takes
 bool fits(nk_ctx* ctx, const GatedCall& c) {
-    if (c.T < 64 || c.H < 64 || c.D < 64 || double(c.T) * double(c.D) * double(c.H) < double(1 << 22)) return false;
+    if (c.H < 64 || c.D < 64 || double(c.T) * double(c.D) * double(c.H) < double(1 << 20)) return false;
     const int64_t most = (int64_t(1) << 21) - 32;
     return c.T < most && c.D < most && c.H < most / 2 && size_t(TcCfg<2, 256>::SMEM_BYTES) <= size_t(ctx->prop.sharedMemPerBlockOptin);
 }
@@ -192,6 +196,10 @@ bool fits(nk_ctx* ctx, const GatedCall& c) {
 int nk_gated_tc_forward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     *handled = false;
     if (!fits(ctx, c)) return NK_OK;
+    if (nk_gated_narrow(ctx, c)) {
+        *handled = true;
+        return nk_gated_narrow_forward(ctx, c);
+    }
     const int64_t Kp = tc_round_k(c.D);
     const TcShape shape = tc_shape(c.T, c.H, Kp, true, ctx->prop.multiProcessorCount);
     Pieces pieces;
@@ -227,18 +235,26 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     *handled = false;
     if (!fits(ctx, c)) return NK_OK;
     const bool dx = c.dx.ptr != nullptr, dw = c.dw[0].ptr || c.dw[1].ptr;
-    const int64_t Hp = tc_round_k(c.H), Tp = tc_round_k(c.T), sms = ctx->prop.multiProcessorCount;
+    // few tokens: dx straight from the weights as they lie (nk_gated_narrow.cu)
+    const bool narrow = nk_gated_narrow(ctx, c);
+    const int64_t Hp = narrow ? nk_gated_narrow_columns(c.H) : tc_round_k(c.H), Tp = tc_round_k(c.T), sms = ctx->prop.multiProcessorCount;
     const TcShape sx = tc_shape(c.T, c.D, 2 * Hp, false, sms), sw = tc_shape(c.D, c.H, Tp, true, sms);
     Pieces pieces;
-    const size_t a_bytes = dx ? size_t(c.T) * 2 * Hp * 4 : 0, w_bytes = dx ? size_t(c.D) * 2 * Hp * 4 : 0;
+    const size_t a_bytes = dx ? size_t(c.T) * 2 * Hp * 4 : 0, w_bytes = dx && !narrow ? size_t(c.D) * 2 * Hp * 4 : 0;
     const size_t e_bytes = dw ? size_t(c.H) * Tp * 4 : 0, x_bytes = dw ? size_t(c.D) * Tp * 4 : 0;
     const size_t a_hi = pieces.take(a_bytes), a_lo = pieces.take(a_bytes), w_hi = pieces.take(w_bytes), w_lo = pieces.take(w_bytes);
     size_t e_at[2][2];
     for (int b = 0; b < 2; b++)
         for (int k = 0; k < 2; k++) e_at[b][k] = pieces.take(e_bytes);
     const size_t x_hi = pieces.take(x_bytes), x_lo = pieces.take(x_bytes);
-    const size_t px = pieces.take(dx ? tc_part_bytes(sx) : 0), pw = pieces.take(dw ? tc_part_bytes(sw) : 0);
-    const size_t tx_bytes = dx ? tc_ticket_bytes(sx) : 0, tw_bytes = dw ? tc_ticket_bytes(sw) : 0;
+    size_t px_bytes = tc_part_bytes(sx), tx_bytes = tc_ticket_bytes(sx);
+    if (narrow) {
+        int n;
+        nk_gated_narrow_dx_needs(ctx, c, &px_bytes, &n);
+        tx_bytes = size_t(n) * sizeof(int);
+    }
+    if (!dx) px_bytes = tx_bytes = 0;
+    const size_t px = pieces.take(px_bytes), pw = pieces.take(dw ? tc_part_bytes(sw) : 0), tw_bytes = dw ? tc_ticket_bytes(sw) : 0;
     const size_t tickets = pieces.take(tx_bytes + tw_bytes);
     NkWorkspace ws(ctx);
     int st = ws.get(pieces.bytes);
@@ -253,6 +269,8 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     for (int b = 0; b < 2 && dw; b++) { ep.t_hi[b] = at(e_at[b][0]); ep.t_lo[b] = at(e_at[b][1]); }
     ep.err_vec = vec_rows(c.err);
     ep.kept_vec = c.H % 4 == 0 && reinterpret_cast<uintptr_t>(c.gate) % 16 == 0 && reinterpret_cast<uintptr_t>(c.up) % 16 == 0;
+    ep.tickets = reinterpret_cast<int*>(at(tickets));
+    ep.n_tickets = int((tx_bytes + tw_bytes) / sizeof(int));
     const int64_t tiles_h = (Hp + 127) / 128, tiles = tiles_h * ((Tp + 31) / 32);
     if (tiles > 0x7fffffffLL) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_gated_grad: an error of more than 2^31 tiles");
 #define NK_CASE(FUN) nk_gated_errors_split_kernel<FUN><<<unsigned(tiles), 256, 0, ctx->stream>>>(c, ep, tiles_h)
@@ -263,7 +281,7 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     TcSplit sp;
     memset(&sp, 0, sizeof(sp));
     int ops = 0;
-    for (int b = 0; b < 2 && dx; b++) {   // [Wg | Wu]: rows d, k = h
+    for (int b = 0; b < 2 && dx && !narrow; b++) {   // [Wg | Wu]: rows d, k = h
         TcOperand& o = sp.op[ops++];
         o = operand(c.w[b].ptr, c.D, c.w[b].rs, c.H, c.w[b].cs);
         tc_operand_layout(&o, c.w[b].cs == 1, at(w_hi) + b * Hp, at(w_lo) + b * Hp, 2 * Hp);
@@ -273,10 +291,10 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
         o = operand(c.x.ptr, c.D, c.x.cs, c.T, c.x.rs);
         tc_operand_layout(&o, c.x.rs == 1, at(x_hi), at(x_lo), Tp);
     }
-    sp.tickets = reinterpret_cast<int*>(at(tickets));
-    sp.n_tickets = int((tx_bytes + tw_bytes) / sizeof(int));
-    if ((st = split(ctx, sp))) return st;
-    if (dx) {
+    if (ops && (st = split(ctx, sp))) return st;
+    if (dx && narrow) {
+        if ((st = nk_gated_narrow_dx(ctx, c, at(a_hi), at(a_lo), at(px), ep.tickets))) return st;
+    } else if (dx) {
         TcPlainDrain drain;
         memset(&drain, 0, sizeof(drain));
         drain.out = static_cast<float*>(c.dx.ptr);
@@ -285,7 +303,7 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
         drain.sOn = c.dx.cs;
         drain.out_vec = vec_rows(c.dx);
         const TcPanels a{at(a_hi), at(a_lo), c.T}, b{at(w_hi), at(w_lo), c.D};
-        if ((st = product(ctx, sx, 2 * Hp, a, b, b, tc_params(sx, c.T, 2 * Hp, at(px), sp.tickets, ctx->tma_status_dev), drain))) return st;
+        if ((st = product(ctx, sx, 2 * Hp, a, b, b, tc_params(sx, c.T, 2 * Hp, at(px), ep.tickets, ctx->tma_status_dev), drain))) return st;
     }
     if (dw) {
         TwoDrain drain;
@@ -298,7 +316,7 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
             drain.vec[b] = vec_rows(c.dw[b]);
         }
         const TcPanels a{at(x_hi), at(x_lo), c.D}, b0{at(e_at[0][0]), at(e_at[0][1]), c.H}, b1{at(e_at[1][0]), at(e_at[1][1]), c.H};
-        st = product(ctx, sw, Tp, a, b0, b1, tc_params(sw, c.D, Tp, at(pw), sp.tickets + tx_bytes / sizeof(int), ctx->tma_status_dev), drain);
+        st = product(ctx, sw, Tp, a, b0, b1, tc_params(sw, c.D, Tp, at(pw), ep.tickets + tx_bytes / sizeof(int), ctx->tma_status_dev), drain);
     }
     *handled = true;
     return st;

@@ -223,6 +223,17 @@ def test_gated_and_its_gradients(device, dtype, size):
     gated_case(device, np.random.default_rng(sum(size)), dtype, *size, "silu")
 
 
+# some tokens: tiles shared by several multiprocessors, chunks and tiles that end inside, one chunk or many per tile
+SOME_SIZES = [(9, 300, 1027), (10, 128, 1024), (16, 1000, 129), (17, 2050, 64), (24, 515, 900), (32, 64, 2048), (33, 130, 2050), (48, 128, 4096), (64, 777, 260), (50, 4100, 70),
+              (12, 66, 20000), (64, 1023, 1025)]
+
+
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("size", SOME_SIZES, ids=str)
+def test_gated_some_tokens(device, size, turned):
+    gated_case(device, np.random.default_rng(sum(size)), np.float32, *size, "silu", ("dense", "turned" if turned else "dense", "turned" if turned else "dense", "dense"))
+
+
 @pytest.mark.parametrize("fun", L.GATES)
 @pytest.mark.parametrize("size", [(1, 70, 90), (5, 64, 48), (24, 200, 136), (200, 300, 260)], ids=str)
 @pytest.mark.parametrize("dtype", TYPES)
