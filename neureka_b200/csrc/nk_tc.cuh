@@ -105,6 +105,7 @@ inline void tc_operand_layout(TcOperand* o, bool kfast, float* hi, float* lo, in
 // 4096^2 operands, two per product: 62 us (58 is the floor); two launches of 32 x 32 tiles with 4-byte accesses: 87 to 114.
 __global__ void __launch_bounds__(256) nk_tc_split_kernel(const TcSplit p) {
     __shared__ float tile[32][129];
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // a launch that allows it may begin what does not need these panels
     int which = 0;
     int64_t t = blockIdx.x;
     while (which + 1 < TC_OPERANDS && t >= p.op[which].tiles) t -= p.op[which++].tiles;
