@@ -1,9 +1,17 @@
 // The gated feed-forward block (no counterpart in the reference):
 //   g = x Wg, u = x Wu, y = f(g) * u;   dg = e * u * f'(g), du = e * f(g), dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du.
 //
-// nk_gated_tile_kernel: any sizes, any strides, both types. Both products of a tile share the panel of x and end in the same thread, so the
-// activation and the product with it happen in registers.
+// Which kernels take a call:
+//   F32  1 token, or a matrix with a side below 16 and at most 8 tokens: nk_gated_few.cu; 2 to 192 tokens: nk_gated_narrow.cu; more, of at least 64 x 64
+//        weights and 2^20 multiply-adds: nk_gated_tc.cu; the rest: nk_gated_tile_kernel;
+//   F64  at most 8 tokens: nk_gated_few.cu; more: nk_gated_dmma_kernel.
+// Both kernels below take any sizes and any strides; both products of a tile share the panel of x and end in the same thread, so the
+// activation and the product with it need no further pass.
+#include <cooperative_groups.h>
+
 #include "nk_gated.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -89,12 +97,157 @@ __global__ void __launch_bounds__(256) nk_gated_tile_kernel(const GatedTile p) {
         }
     }
 }
+// ---- F64 on the FP64 matrix instructions -----------------------------------------------------------------------------------------
+// mma.m8n8k4, 64 x 64 tiles of four warps with 32 x 32 each (nk_conv_gemm.cu: why). With two B operands the tile is 32 columns of each product and
+// the blocks of eight columns alternate between the two, so that a thread holds both products of an element. k is split over the CTAs of a
+// cluster where the tiles are few; the tile passes through shared memory at the end, where the cluster's parts meet in rank order.
+constexpr int GD_T = 64, GD_K = 16, GD_PITCH = 20;   // a panel's rows have a pitch of 20 doubles: the fragment loads of a half warp fall on 16 banks
+__device__ __forceinline__ void gd_mma(double (&c)[2], double a, double b) {
+    asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
+}
+template <int MODE>
+__global__ void __launch_bounds__(128, 3) nk_gated_dmma_kernel(const GatedTile p) {
+    constexpr int COLS = MODE == GATED_SUM ? GD_T : GD_T / 2;   // columns of an output that a tile covers
+    __shared__ double smem[2 * 2 * GD_T * GD_PITCH];            // [buffer][A, B][row][k]; then the tile, [row][column]
+    auto As = reinterpret_cast<double (*)[2][GD_T][GD_PITCH]>(smem);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int size = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int64_t tiles_n = (p.N + COLS - 1) / COLS, t = blockIdx.x / unsigned(size);
+    const int64_t m0 = (t / tiles_n) * GD_T, n0 = (t % tiles_n) * COLS;
+    // panels of 16 k, of both phases of a SUM one after the other; this CTA's share of them
+    const int64_t phase_panels = (p.K + GD_K - 1) / GD_K, panels = phase_panels * (MODE == GATED_SUM ? 2 : 1);
+    const int64_t first = rank * panels / size, last = (rank + 1) * panels / size;
+    double ra[8], rb[8];
+    // element i of a thread's share of a panel, the operand's contiguous direction across the threads
+    auto place = [&](bool kfast, int i, int* r, int* k) {
+        if (kfast) { *k = tid & 15; *r = (tid >> 4) + 8 * i; }
+        else { *r = tid & 63; *k = (tid >> 6) + 2 * i; }
+    };
+    auto fetch = [&](int64_t panel) {
+        const int phase = MODE == GATED_SUM && panel >= phase_panels;
+        const int64_t k0 = (panel - phase * phase_panels) * GD_K;
+        const GatedMatrix& A = p.a[phase];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            int r, k;
+            place(A.cs == 1, i, &r, &k);
+            ra[i] = m0 + r < p.M && k0 + k < p.K ? static_cast<const double*>(A.ptr)[(m0 + r) * A.rs + (k0 + k) * A.cs] : 0.0;
+            place(p.b[phase].rs == 1, i, &r, &k);
+            const int which = MODE == GATED_SUM ? phase : (r >> 3) & 1;
+            const int64_t c = n0 + (MODE == GATED_SUM ? r : (r >> 4) * 8 + (r & 7));
+            const GatedMatrix& B = p.b[which];
+            rb[i] = c < p.N && k0 + k < p.K ? static_cast<const double*>(B.ptr)[(k0 + k) * B.rs + c * B.cs] : 0.0;
+        }
+    };
+    auto stash = [&](int64_t panel, int buf) {
+        const int phase = MODE == GATED_SUM && panel >= phase_panels;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            int r, k;
+            place(p.a[phase].cs == 1, i, &r, &k);
+            As[buf][0][r][k] = ra[i];
+            place(p.b[phase].rs == 1, i, &r, &k);
+            As[buf][1][r][k] = rb[i];
+        }
+    };
+    double acc[4][4][2];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][j][0] = acc[i][j][1] = 0.0;
+    const int wm = (warp >> 1) * 32, wn = (warp & 1) * 32, fr = lane >> 2, fk = lane & 3;
+    if (first < last) {
+        fetch(first);
+        stash(first, 0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int64_t panel = first; panel < last; panel++) {
+        const bool more = panel + 1 < last;
+        if (more) fetch(panel + 1);
+#pragma unroll
+        for (int k = 0; k < GD_K; k += 4) {
+            double a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) a[i] = As[buf][0][wm + 8 * i + fr][k + fk];
+#pragma unroll
+            for (int j = 0; j < 4; j++) b[j] = As[buf][1][wn + 8 * j + fr][k + fk];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) gd_mma(acc[i][j], a[i], b[j]);
+        }
+        if (more) {
+            stash(panel + 1, buf ^ 1);   // the other buffer was last read one panel ago, before the barrier below
+            __syncthreads();
+            buf ^= 1;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) *reinterpret_cast<double2*>(smem + (wm + 8 * i + fr) * GD_T + wn + 8 * j + 2 * fk) = make_double2(acc[i][j][0], acc[i][j][1]);
+    cluster.sync();   // (a CTA alone: a barrier)
+    for (int e = rank * 128 + tid; e < GD_T * COLS; e += size * 128) {
+        const int r = e / COLS, c = e % COLS;
+        const int64_t m = m0 + r, n = n0 + c;
+        if (m >= p.M || n >= p.N) continue;
+        const int at = r * GD_T + (MODE == GATED_SUM ? c : (c >> 3) * 16 + (c & 7));
+        double v[2] = {0.0, 0.0};
+        for (int q = 0; q < size; q++) {
+            const double* theirs = cluster.map_shared_rank(smem, q);
+            v[0] += theirs[at];
+            if (MODE != GATED_SUM) v[1] += theirs[at + 8];
+        }
+        if (MODE == GATED_FORWARD) {
+            if (p.gate) {
+                static_cast<double*>(p.gate)[m * p.N + n] = v[0];
+                static_cast<double*>(p.up)[m * p.N + n] = v[1];
+            }
+            static_cast<double*>(p.out[0].ptr)[m * p.out[0].rs + n * p.out[0].cs] = gate_fun<double>(p.fun, false, v[0]) * v[1];
+        } else {
+#pragma unroll
+            for (int b = 0; b < (MODE == GATED_SUM ? 1 : 2); b++)
+                if (p.out[b].ptr) static_cast<double*>(p.out[b].ptr)[m * p.out[b].rs + n * p.out[b].cs] = v[b];
+        }
+    }
+    if (size > 1) cluster.sync();   // nobody leaves while its part may still be read
+}
+template <int MODE>
+int launch_dmma(nk_ctx* ctx, const GatedTile& p) {
+    constexpr int COLS = MODE == GATED_SUM ? GD_T : GD_T / 2;
+    const int64_t tiles = ((p.M + GD_T - 1) / GD_T) * ((p.N + COLS - 1) / COLS), panels = (p.K + GD_K - 1) / GD_K * (MODE == GATED_SUM ? 2 : 1);
+    // three CTAs fit an SM: k is split, in parts of at least 64, until there are about two per SM
+    int split = 1;
+    while (split < 8 && tiles * split < int64_t(ctx->prop.multiProcessorCount) * 2 && panels / (split * 2) >= 4) split *= 2;
+    if (tiles * split > 0x7fffffffLL) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_gated: a result of %lld x %lld elements is too large", (long long)p.M, (long long)p.N);
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(unsigned(tiles * split));
+    cfg.blockDim = dim3(128);
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(split);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = split > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, nk_gated_dmma_kernel<MODE>, p);
+    if (e != cudaSuccess) return nk_cuda_fail(ctx, e, "nk_gated_dmma_kernel");
+    return nk_after_launch(ctx, "nk_gated_dmma_kernel");
+}
+
 template <class T, int MODE>
 int launch_tiles(nk_ctx* ctx, const GatedTile& p) {
-    const int64_t tiles = ((p.M + GT - 1) / GT) * ((p.N + GT - 1) / GT);
-    if (tiles > 0x7fffffffLL) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_gated: a result of %lld x %lld elements is too large", (long long)p.M, (long long)p.N);
-    nk_gated_tile_kernel<T, MODE><<<unsigned(tiles), 256, 0, ctx->stream>>>(p);
-    return nk_after_launch(ctx, "nk_gated_tile_kernel");
+    if constexpr (sizeof(T) == 8) return launch_dmma<MODE>(ctx, p);
+    else {
+        const int64_t tiles = ((p.M + GT - 1) / GT) * ((p.N + GT - 1) / GT);
+        if (tiles > 0x7fffffffLL) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_gated: a result of %lld x %lld elements is too large", (long long)p.M, (long long)p.N);
+        nk_gated_tile_kernel<T, MODE><<<unsigned(tiles), 256, 0, ctx->stream>>>(p);
+        return nk_after_launch(ctx, "nk_gated_tile_kernel");
+    }
 }
 
 // dg and du, row-major [T, H]
@@ -113,12 +266,13 @@ GatedMatrix turned(const GatedMatrix& m) { return GatedMatrix{m.ptr, m.cs, m.rs}
 
 template <class T>
 int forward(nk_ctx* ctx, const GatedCall& c) {
-    if (nk_gated_few(c)) return nk_gated_few_forward<T>(ctx, c);
-    if (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4) {
+        if (c.T > 1 && nk_gated_narrow(ctx, c)) return nk_gated_narrow_forward(ctx, c);
         bool handled = false;
         const int st = nk_gated_tc_forward(ctx, c, &handled);
         if (st || handled) return st;
     }
+    if (c.T <= nk_gated_few_most()) return nk_gated_few_forward<T>(ctx, c);
     GatedTile p;
     memset(&p, 0, sizeof(p));
     p.fun = c.fun;
@@ -142,11 +296,23 @@ int backward(nk_ctx* ctx, const GatedCall& c) {
     T *dg = static_cast<T*>(ws.ptr), *du = dg + c.T * c.H;
     nk_gated_errors_kernel<T><<<nk_grid_for(ctx, c.T * c.H, 256, 8), 256, 0, ctx->stream>>>(c, dg, du);
     if ((st = nk_after_launch(ctx, "nk_gated_errors_kernel"))) return st;
-    if (nk_gated_few(c)) return nk_gated_few_backward<T>(ctx, c, dg, du);
+    if (c.T <= nk_gated_few_most()) {
+        if (c.dx.ptr) {
+            if constexpr (sizeof(T) == 4) st = c.T > 1 && nk_gated_narrow(ctx, c) ? nk_gated_narrow_dx(ctx, c, dg, du) : nk_gated_few_dx<T>(ctx, c, dg, du);
+            else st = nk_gated_few_dx<T>(ctx, c, dg, du);
+            if (st) return st;
+        }
+        return c.dw[0].ptr || c.dw[1].ptr ? nk_gated_few_dw<T>(ctx, c, dg, du) : int(NK_OK);
+    }
     const GatedMatrix mg{dg, c.H, 1}, mu{du, c.H, 1};
     GatedTile p;
     memset(&p, 0, sizeof(p));
-    if (c.dx.ptr) {
+    bool narrow = false;
+    if constexpr (sizeof(T) == 4) {
+        narrow = c.dx.ptr && nk_gated_narrow(ctx, c);
+        if (narrow && (st = nk_gated_narrow_dx(ctx, c, dg, du))) return st;
+    }
+    if (c.dx.ptr && !narrow) {
         p.M = c.T; p.N = c.D; p.K = c.H;
         p.a[0] = mg; p.a[1] = mu;
         p.b[0] = turned(c.w[0]); p.b[1] = turned(c.w[1]);

@@ -47,14 +47,17 @@ __device__ __forceinline__ T gate_fun(int f, bool derive, T x) {
 int nk_gated_tc_forward(nk_ctx* ctx, const GatedCall& c, bool* handled);
 int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled);
 
-// Few tokens, both types (nk_gated_few.cu). dg and du: row-major [T, H].
-bool nk_gated_few(const GatedCall& c);
+// Few tokens, at most nk_gated_few_most(), both types (nk_gated_few.cu). dg and du: row-major [T, H].
+int64_t nk_gated_few_most();
 template <class T> int nk_gated_few_forward(nk_ctx* ctx, const GatedCall& c);
-template <class T> int nk_gated_few_backward(nk_ctx* ctx, const GatedCall& c, const T* dg, const T* du);
+template <class T> int nk_gated_few_dx(nk_ctx* ctx, const GatedCall& c, const T* dg, const T* du);
+template <class T> int nk_gated_few_dw(nk_ctx* ctx, const GatedCall& c, const T* dg, const T* du);
 
-// Some tokens in F32 (nk_gated_narrow.cu). dx: hi and lo are panels [T][2 * nk_gated_narrow_columns(H)] of dg and du, zero past H; the tickets are zero.
+// Some tokens in F32 (nk_gated_narrow.cu). dx from dg and du, or from panels hi and lo [T][2 * nk_gated_narrow_columns(H)] of them, zero past H, and
+// cleared tickets.
 bool nk_gated_narrow(const nk_ctx* ctx, const GatedCall& c);
 int nk_gated_narrow_forward(nk_ctx* ctx, const GatedCall& c);
 int64_t nk_gated_narrow_columns(int64_t H);
 void nk_gated_narrow_dx_needs(nk_ctx* ctx, const GatedCall& c, size_t* part_bytes, int* tickets);
-int nk_gated_narrow_dx(nk_ctx* ctx, const GatedCall& c, const float* hi, const float* lo, float* parts, int* tickets);
+int nk_gated_narrow_dx(nk_ctx* ctx, const GatedCall& c, const float* dg, const float* du);
+int nk_gated_narrow_dx_panels(nk_ctx* ctx, const GatedCall& c, const float* hi, const float* lo, float* parts, int* tickets);

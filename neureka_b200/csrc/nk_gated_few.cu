@@ -15,7 +15,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32, FEW_MAX = 8, FEW_K = 512;   // k per chunk of a slice
+constexpr int FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32, FEW_MAX = 8, FEW_K = 512, FEW_SLICE = 128;   // k per chunk of a slice; a slice is a multiple of
 template <class T, int W> struct FewVec { using type = T; };
 template <> struct FewVec<float, 4> { using type = float4; };
 template <> struct FewVec<double, 2> { using type = double2; };
@@ -24,7 +24,7 @@ template <class T> constexpr int few_v = 16 / int(sizeof(T));
 struct FewCall {
     int fun;
     int tokens;
-    int64_t N, K, slice;      // columns of the result, length of the sums, k per CTA (a multiple of FEW_K, or K)
+    int64_t N, K, slice;      // columns of the result, length of the sums, k per CTA (a multiple of FEW_SLICE)
     GatedMatrix x[2];         // [tokens, K]; SUM: dg and du
     GatedMatrix w[2];         // [K, N]
     GatedMatrix out;          // [tokens, N]
@@ -270,11 +270,11 @@ template <class T, int TOK, bool TURNED, bool VEC, bool SUM>
 int few_launch(nk_ctx* ctx, FewCall p) {
     constexpr int COLS = 32 * few_v<T>;
     constexpr size_t smem = sizeof(T) * TOK * ((SUM ? 2 : 1) * FEW_K + (SUM ? 1 : 2) * COLS);
-    // k is split until there are about four CTAs per SM, at most eight ways (a portable cluster), each of at least a chunk
-    const int64_t tiles = (p.N + COLS - 1) / COLS, chunks = (p.K + FEW_K - 1) / FEW_K;
+    // k is split until there are about four CTAs per SM, at most eight ways (a portable cluster)
+    const int64_t tiles = (p.N + COLS - 1) / COLS, pieces = (p.K + FEW_SLICE - 1) / FEW_SLICE;
     int split = 1;
-    while (split < 8 && split < chunks && tiles * split < int64_t(ctx->prop.multiProcessorCount) * 3) split *= 2;
-    p.slice = (chunks + split - 1) / split * FEW_K;
+    while (split < 8 && split < pieces && tiles * split < int64_t(ctx->prop.multiProcessorCount) * 3) split *= 2;
+    p.slice = (pieces + split - 1) / split * FEW_SLICE;
     if (tiles * split > 0x7fffffffLL) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_gated: a result of %lld columns is too large", (long long)p.N);
     auto* kern = nk_gated_few_kernel<T, TOK, TURNED, VEC, SUM>;
     if (smem > 48 * 1024) NK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
@@ -298,7 +298,7 @@ template <class T, int TOK, bool SUM>
 int few_route(nk_ctx* ctx, const FewCall& p) {
     const bool turned = p.w[0].rs == 1 && p.w[1].rs == 1 && p.w[0].cs != 1;
     if (turned) {
-        // (the slices start at multiples of FEW_K: only K itself and the weights decide whether vectors fit)
+        // (the slices start at multiples of FEW_SLICE: only K itself and the weights decide whether vectors fit)
         if (p.K % few_v<T> == 0 && few_aligned<T>(p.w[0], false) && few_aligned<T>(p.w[1], false)) return few_launch<T, TOK, true, true, SUM>(ctx, p);
         return few_launch<T, TOK, true, false, SUM>(ctx, p);
     }
@@ -325,7 +325,7 @@ int outer_launch(nk_ctx* ctx, const OuterCall& p) {
 
 }  // namespace
 
-bool nk_gated_few(const GatedCall& c) { return c.T <= FEW_MAX; }
+int64_t nk_gated_few_most() { return FEW_MAX; }
 
 template <class T>
 int nk_gated_few_forward(nk_ctx* ctx, const GatedCall& c) {
@@ -344,21 +344,20 @@ int nk_gated_few_forward(nk_ctx* ctx, const GatedCall& c) {
     return few_tokens<T, false>(ctx, p);
 }
 template <class T>
-int nk_gated_few_backward(nk_ctx* ctx, const GatedCall& c, const T* dg, const T* du) {
-    int st;
-    if (c.dx.ptr) {
-        FewCall p;
-        memset(&p, 0, sizeof(p));
-        p.tokens = int(c.T);
-        p.N = c.D;
-        p.K = c.H;
-        p.x[0] = GatedMatrix{const_cast<T*>(dg), c.H, 1};
-        p.x[1] = GatedMatrix{const_cast<T*>(du), c.H, 1};
-        for (int b = 0; b < 2; b++) p.w[b] = GatedMatrix{c.w[b].ptr, c.w[b].cs, c.w[b].rs};
-        p.out = c.dx;
-        if ((st = few_tokens<T, true>(ctx, p))) return st;
-    }
-    if (!c.dw[0].ptr && !c.dw[1].ptr) return NK_OK;
+int nk_gated_few_dx(nk_ctx* ctx, const GatedCall& c, const T* dg, const T* du) {
+    FewCall p;
+    memset(&p, 0, sizeof(p));
+    p.tokens = int(c.T);
+    p.N = c.D;
+    p.K = c.H;
+    p.x[0] = GatedMatrix{const_cast<T*>(dg), c.H, 1};
+    p.x[1] = GatedMatrix{const_cast<T*>(du), c.H, 1};
+    for (int b = 0; b < 2; b++) p.w[b] = GatedMatrix{c.w[b].ptr, c.w[b].cs, c.w[b].rs};
+    p.out = c.dx;
+    return few_tokens<T, true>(ctx, p);
+}
+template <class T>
+int nk_gated_few_dw(nk_ctx* ctx, const GatedCall& c, const T* dg, const T* du) {
     OuterCall o;
     memset(&o, 0, sizeof(o));
     o.tokens = int(c.T);
@@ -374,5 +373,7 @@ int nk_gated_few_backward(nk_ctx* ctx, const GatedCall& c, const T* dg, const T*
 }
 template int nk_gated_few_forward<float>(nk_ctx*, const GatedCall&);
 template int nk_gated_few_forward<double>(nk_ctx*, const GatedCall&);
-template int nk_gated_few_backward<float>(nk_ctx*, const GatedCall&, const float*, const float*);
-template int nk_gated_few_backward<double>(nk_ctx*, const GatedCall&, const double*, const double*);
+template int nk_gated_few_dx<float>(nk_ctx*, const GatedCall&, const float*, const float*);
+template int nk_gated_few_dx<double>(nk_ctx*, const GatedCall&, const double*, const double*);
+template int nk_gated_few_dw<float>(nk_ctx*, const GatedCall&, const float*, const float*);
+template int nk_gated_few_dw<double>(nk_ctx*, const GatedCall&, const double*, const double*);

@@ -509,7 +509,9 @@ int narrow(nk_ctx* ctx, const NarrowCall& p, const float* hi, const float* lo, i
 }  // namespace
 
 bool nk_gated_narrow(const nk_ctx* ctx, const GatedCall& c) {
-    if (c.T > 64) return false;
+    // Up to three tiles of 64 tokens: every tile reads the weights again (64 tokens 84 us at 4096 x 8192), where panels of them (nk_gated_tc.cu) cost
+    // their split, 150 us there, and 1.1 us per token.
+    if (c.T > 192 || c.D < 16 || c.H < 16) return false;
     const int64_t most = int64_t(1) << 30;
     return c.D < most && c.H < most && double(c.D) * double(c.H) < 4e12 && size_t(NarrowCfg<64, false>::SMEM) <= size_t(ctx->prop.sharedMemPerBlockOptin);
 }
@@ -568,9 +570,35 @@ void nk_gated_narrow_dx_needs(nk_ctx* ctx, const GatedCall& c, size_t* part_byte
     *part_bytes = narrow_part_bytes(ctx, p, true);
     *tickets = p.tiles;
 }
-int nk_gated_narrow_dx(nk_ctx* ctx, const GatedCall& c, const float* hi, const float* lo, float* parts, int* tickets) {
+int nk_gated_narrow_dx_panels(nk_ctx* ctx, const GatedCall& c, const float* hi, const float* lo, float* parts, int* tickets) {
     NarrowCall p = narrow_dx_call(ctx, c);
     p.parts = parts;
     p.tickets = tickets;
     return narrow<true>(ctx, p, hi, lo, 2 * p.Kq);
+}
+int nk_gated_narrow_dx(nk_ctx* ctx, const GatedCall& c, const float* dg, const float* du) {
+    const NarrowCall p = narrow_dx_call(ctx, c);
+    auto pad = [](size_t b) { return (b + 1023) / 1024 * 1024; };
+    const size_t e_bytes = pad(size_t(c.T) * 2 * p.Kq * 4), part_bytes = pad(narrow_part_bytes(ctx, p, true));
+    NkWorkspace ws(ctx);
+    int st = ws.get(2 * e_bytes + part_bytes + size_t(p.tiles) * sizeof(int));
+    if (st) return st;
+    char* base = static_cast<char*>(ws.ptr);
+    float *hi = reinterpret_cast<float*>(base), *lo = reinterpret_cast<float*>(base + e_bytes);
+    int* tickets = reinterpret_cast<int*>(base + 2 * e_bytes + part_bytes);
+    TcSplit sp;
+    memset(&sp, 0, sizeof(sp));
+    int64_t tiles = 0;
+    for (int b = 0; b < 2; b++) {
+        TcOperand& o = sp.op[b];
+        o.src = b ? du : dg;
+        o.R = c.T; o.sR = c.H; o.K = c.H; o.sK = 1;
+        tc_operand_layout(&o, true, hi + b * p.Kq, lo + b * p.Kq, 2 * p.Kq, p.Kq);
+        tiles += o.tiles;
+    }
+    sp.tickets = tickets;
+    sp.n_tickets = p.tiles;
+    nk_tc_split_kernel<<<unsigned(tiles), 256, 0, ctx->stream>>>(sp);
+    if ((st = nk_after_launch(ctx, "nk_tc_split_kernel"))) return st;
+    return nk_gated_narrow_dx_panels(ctx, c, hi, lo, reinterpret_cast<float*>(base + 2 * e_bytes), tickets);
 }

@@ -11,36 +11,41 @@
 
 namespace {
 
+// eight values of a row: one 32-byte store fills its sector (rows of a tile are apart, so two of 16 bytes reach L2 as two halves)
+__device__ __forceinline__ void store8(float* at, const float* v) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(at), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]),
+                 "f"(v[7]) : "memory");
+}
 // f(g) * u, and g and u where they are kept
 template <int FUN>
 struct GatedDrain {
     static constexpr bool DUAL = true;
     float *y, *gate, *up;
     int64_t N, rs, cs;
-    int vec, kept_vec;   // 16-byte stores: the rows of y; of gate and up
+    int vec, kept_vec;   // 32-byte stores: the rows of y; of gate and up
     template <int EC>
     __device__ __forceinline__ void store(int64_t m, int64_t n0, const float (&sum)[EC]) const {
         constexpr int HC = EC / 2;
 #pragma unroll
-        for (int j = 0; j < HC; j += 4) {
+        for (int j = 0; j < HC; j += 8) {
             const int64_t n = n0 + j;
             if (n >= N) continue;
-            float v[4];
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = nkf::fun(FUN, false, sum[j + i]) * sum[HC + j + i];
-            if (vec && n + 4 <= N) *reinterpret_cast<float4*>(y + m * rs + n) = make_float4(v[0], v[1], v[2], v[3]);
+            for (int i = 0; i < 8; i++) v[i] = nkf::fun(FUN, false, sum[j + i]) * sum[HC + j + i];
+            if (vec && n + 8 <= N) store8(y + m * rs + n, v);
             else {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 8; i++)
                     if (n + i < N) y[m * rs + (n + i) * cs] = v[i];
             }
             if (!gate) continue;
             if (kept_vec) {
-                *reinterpret_cast<float4*>(gate + m * N + n) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
-                *reinterpret_cast<float4*>(up + m * N + n) = make_float4(sum[HC + j], sum[HC + j + 1], sum[HC + j + 2], sum[HC + j + 3]);
+                store8(gate + m * N + n, sum + j);
+                store8(up + m * N + n, sum + HC + j);
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 8; i++)
                     if (n + i < N) { gate[m * N + n + i] = sum[j + i]; up[m * N + n + i] = sum[HC + j + i]; }
             }
         }
@@ -51,7 +56,7 @@ struct TwoDrain {
     static constexpr bool DUAL = true;
     float* out[2];
     int64_t N, rs[2], cs[2];
-    int vec[2];
+    int vec[2];          // 32-byte stores along the rows
     template <int EC>
     __device__ __forceinline__ void store(int64_t m, int64_t n0, const float (&sum)[EC]) const {
         constexpr int HC = EC / 2;
@@ -60,14 +65,14 @@ struct TwoDrain {
             if (!out[b]) continue;
             float* row = out[b] + m * rs[b];
 #pragma unroll
-            for (int j = 0; j < HC; j += 4) {
+            for (int j = 0; j < HC; j += 8) {
                 const int64_t n = n0 + j;
                 if (n >= N) continue;
                 const float* v = sum + b * HC + j;
-                if (vec[b] && n + 4 <= N) *reinterpret_cast<float4*>(row + n) = make_float4(v[0], v[1], v[2], v[3]);
+                if (vec[b] && n + 8 <= N) store8(row + n, v);
                 else {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                    for (int i = 0; i < 8; i++)
                         if (n + i < N) row[(n + i) * cs[b]] = v[i];
                 }
             }
@@ -153,6 +158,7 @@ __global__ void __launch_bounds__(256) nk_gated_errors_split_kernel(const GatedC
     }
 }
 
+bool wide_rows(const GatedMatrix& m) { return m.cs == 1 && m.rs % 8 == 0 && reinterpret_cast<uintptr_t>(m.ptr) % 32 == 0; }
 bool vec_rows(const GatedMatrix& m) { return m.cs == 1 && m.rs % 4 == 0 && reinterpret_cast<uintptr_t>(m.ptr) % 16 == 0; }
 // [R, K] of a matrix's view: rows at row_stride, k at k_stride
 TcOperand operand(const void* src, int64_t R, int64_t sR, int64_t K, int64_t sK) {
@@ -186,7 +192,7 @@ int product(nk_ctx* ctx, const TcShape& shape, int64_t Kp, const TcPanels& a, co
 }
 // sizes that the tensor-core path takes
 bool fits(nk_ctx* ctx, const GatedCall& c) {
-    if (c.H < 64 || c.D < 64 || double(c.T) * double(c.D) * double(c.H) < double(1 << 20)) return false;
+    if (c.T <= nk_gated_few_most() || c.H < 64 || c.D < 64 || double(c.T) * double(c.D) * double(c.H) < double(1 << 20)) return false;
     const int64_t most = (int64_t(1) << 21) - 32;
     return c.T < most && c.D < most && c.H < most / 2 && size_t(TcCfg<2, 256>::SMEM_BYTES) <= size_t(ctx->prop.sharedMemPerBlockOptin);
 }
@@ -196,10 +202,6 @@ bool fits(nk_ctx* ctx, const GatedCall& c) {
 int nk_gated_tc_forward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     *handled = false;
     if (!fits(ctx, c)) return NK_OK;
-    if (nk_gated_narrow(ctx, c)) {
-        *handled = true;
-        return nk_gated_narrow_forward(ctx, c);
-    }
     const int64_t Kp = tc_round_k(c.D);
     const TcShape shape = tc_shape(c.T, c.H, Kp, true, ctx->prop.multiProcessorCount);
     Pieces pieces;
@@ -223,8 +225,8 @@ int nk_gated_tc_forward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     if ((st = split(ctx, sp))) return st;
     const TcParams tp = tc_params(shape, c.T, Kp, at(parts), sp.tickets, ctx->tma_status_dev);
     const TcPanels a{at(x_hi), at(x_lo), c.T}, b0{at(g_hi), at(g_lo), c.H}, b1{at(u_hi), at(u_lo), c.H};
-    const int kept_vec = c.H % 4 == 0 && reinterpret_cast<uintptr_t>(c.gate) % 16 == 0 && reinterpret_cast<uintptr_t>(c.up) % 16 == 0;
-#define NK_CASE(FUN) st = product(ctx, shape, Kp, a, b0, b1, tp, GatedDrain<FUN>{static_cast<float*>(c.y.ptr), static_cast<float*>(c.gate), static_cast<float*>(c.up), c.H, c.y.rs, c.y.cs, vec_rows(c.y), kept_vec})
+    const int kept_vec = c.H % 8 == 0 && reinterpret_cast<uintptr_t>(c.gate) % 32 == 0 && reinterpret_cast<uintptr_t>(c.up) % 32 == 0;
+#define NK_CASE(FUN) st = product(ctx, shape, Kp, a, b0, b1, tp, GatedDrain<FUN>{static_cast<float*>(c.y.ptr), static_cast<float*>(c.gate), static_cast<float*>(c.up), c.H, c.y.rs, c.y.cs, wide_rows(c.y), kept_vec})
     NK_GATE_SWITCH(c.fun, NK_CASE)
 #undef NK_CASE
     *handled = true;
@@ -293,7 +295,7 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     }
     if (ops && (st = split(ctx, sp))) return st;
     if (dx && narrow) {
-        if ((st = nk_gated_narrow_dx(ctx, c, at(a_hi), at(a_lo), at(px), ep.tickets))) return st;
+        if ((st = nk_gated_narrow_dx_panels(ctx, c, at(a_hi), at(a_lo), at(px), ep.tickets))) return st;
     } else if (dx) {
         TcPlainDrain drain;
         memset(&drain, 0, sizeof(drain));
@@ -313,7 +315,7 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
             drain.out[b] = static_cast<float*>(c.dw[b].ptr);
             drain.rs[b] = c.dw[b].rs;
             drain.cs[b] = c.dw[b].cs;
-            drain.vec[b] = vec_rows(c.dw[b]);
+            drain.vec[b] = wide_rows(c.dw[b]);
         }
         const TcPanels a{at(x_hi), at(x_lo), c.D}, b0{at(e_at[0][0]), at(e_at[0][1]), c.H}, b1{at(e_at[1][0]), at(e_at[1][1]), c.H};
         st = product(ctx, sw, Tp, a, b0, b1, tc_params(sw, c.D, Tp, at(pw), ep.tickets + tx_bytes / sizeof(int), ctx->tma_status_dev), drain);

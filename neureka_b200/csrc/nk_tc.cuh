@@ -73,7 +73,7 @@ __device__ __forceinline__ void tc_split(float v, float* hi, float* lo) {
 struct TcOperand {
     const float* src;             // the view's base
     const int64_t *offR, *offK;   // null: r * sR, k * sK
-    int64_t sR, sK, R, K, Kp;     // Kp: K rounded up to 16
+    int64_t sR, sK, R, K, Kp;     // Kp: columns of the panel, a multiple of 16, zero from K on
     int64_t pitch;                // of a row of hi and lo; Kp unless several operands lie side by side along k
     int64_t tiles;                // CTAs for this operand
     int kfast;                    // consecutive k are consecutive in memory
@@ -87,9 +87,10 @@ struct TcSplit {
     int n_tickets;
 };
 inline int64_t tc_round_k(int64_t k) { return (k + TC_BK - 1) / TC_BK * TC_BK; }
-// src, offsets, strides, R and K are there; the rest follows. kfast: the operand's contiguous direction is k.
-inline void tc_operand_layout(TcOperand* o, bool kfast, float* hi, float* lo, int64_t pitch) {
-    o->Kp = tc_round_k(o->K);
+// src, offsets, strides, R and K are there; the rest follows. kfast: the operand's contiguous direction is k. columns: Kp, where more of a panel than
+// up to the next multiple of 16 has to be zero.
+inline void tc_operand_layout(TcOperand* o, bool kfast, float* hi, float* lo, int64_t pitch, int64_t columns = 0) {
+    o->Kp = columns ? columns : tc_round_k(o->K);
     o->pitch = pitch;
     o->hi = hi;
     o->lo = lo;
