@@ -119,36 +119,67 @@ __global__ void __launch_bounds__(128, 3) nk_gated_dmma_kernel(const GatedTile p
     const int64_t phase_panels = (p.K + GD_K - 1) / GD_K, panels = phase_panels * (MODE == GATED_SUM ? 2 : 1);
     const int64_t first = rank * panels / size, last = (rank + 1) * panels / size;
     double ra[8], rb[8];
-    // element i of a thread's share of a panel, the operand's contiguous direction across the threads
-    auto place = [&](bool kfast, int i, int* r, int* k) {
-        if (kfast) { *k = tid & 15; *r = (tid >> 4) + 8 * i; }
-        else { *r = tid & 63; *k = (tid >> 6) + 2 * i; }
+    // Element i of a thread's share of a panel, the operand's contiguous direction across the threads: k = tid % 16 and rows tid / 16 + 8 i where k is,
+    // otherwise row tid % 64 and k = tid / 64 + 2 i. An element's address is one base per thread plus a constant step, moved on by a
+    // panel at a time (worked out per element, the integer chains took longer than the products).
+    struct Walk {
+        const double* at;
+        int64_t step, panel;
+        unsigned rows;   // bit i: element i's row exists
+    };
+    bool a_kfast = false, b_kfast = false;
+    Walk wa, wb[2];      // two B operands, k contiguous: the even elements' and the odd ones'
+    auto walk = [&](const GatedMatrix& m, int64_t rs, int64_t ks, bool kfast, int64_t row0, int64_t rows, int stride, int n, int64_t k0) {
+        Walk w;
+        const int r = kfast ? tid >> 4 : tid & 63, k = kfast ? tid & 15 : tid >> 6;
+        w.at = static_cast<const double*>(m.ptr) + (row0 + r) * rs + (k0 + k) * ks;
+        w.step = kfast ? stride * rs : 2 * ks;
+        w.panel = GD_K * ks;
+        w.rows = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < n && row0 + r + (kfast ? stride * i : 0) < rows) w.rows |= 1u << i;
+        return w;
+    };
+    auto start = [&](int phase, int64_t k0) {
+        const GatedMatrix& A = p.a[phase];
+        a_kfast = A.cs == 1;
+        wa = walk(A, A.rs, A.cs, a_kfast, m0, p.M, 8, 8, k0);
+        b_kfast = p.b[phase].rs == 1;
+        if (MODE == GATED_SUM) {
+            wb[0] = walk(p.b[phase], p.b[phase].cs, p.b[phase].rs, b_kfast, n0, p.N, 8, 8, k0);
+        } else if (b_kfast) {   // rows tid / 16 + 8 i of the panel: column tid / 16 + 8 (i / 2) of operand i % 2
+#pragma unroll
+            for (int w = 0; w < 2; w++) wb[w] = walk(p.b[w], p.b[w].cs, p.b[w].rs, true, n0, p.N, 8, 4, k0);
+        } else {                // row tid % 64: column 8 (row / 16) + row % 8 of operand (row / 8) % 2
+            const int r = tid & 63;
+            const GatedMatrix& B = p.b[(r >> 3) & 1];
+            wb[0] = walk(B, B.cs, B.rs, false, n0 + (r >> 4) * 8 + (r & 7) - r, p.N, 8, 8, k0);
+        }
     };
     auto fetch = [&](int64_t panel) {
         const int phase = MODE == GATED_SUM && panel >= phase_panels;
         const int64_t k0 = (panel - phase * phase_panels) * GD_K;
-        const GatedMatrix& A = p.a[phase];
+        if (panel == first || (MODE == GATED_SUM && panel == phase_panels)) start(phase, k0);
+        const int left = p.K - k0 < GD_K ? int(p.K - k0) : GD_K, ak = a_kfast ? tid & 15 : tid >> 6, bk = b_kfast ? tid & 15 : tid >> 6;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            int r, k;
-            place(A.cs == 1, i, &r, &k);
-            ra[i] = m0 + r < p.M && k0 + k < p.K ? static_cast<const double*>(A.ptr)[(m0 + r) * A.rs + (k0 + k) * A.cs] : 0.0;
-            place(p.b[phase].rs == 1, i, &r, &k);
-            const int which = MODE == GATED_SUM ? phase : (r >> 3) & 1;
-            const int64_t c = n0 + (MODE == GATED_SUM ? r : (r >> 4) * 8 + (r & 7));
-            const GatedMatrix& B = p.b[which];
-            rb[i] = c < p.N && k0 + k < p.K ? static_cast<const double*>(B.ptr)[(k0 + k) * B.rs + c * B.cs] : 0.0;
+        for (int i = 0; i < 8; i++) ra[i] = ((wa.rows >> i) & 1u) && ak + (a_kfast ? 0 : 2 * i) < left ? wa.at[i * wa.step] : 0.0;
+        wa.at += wa.panel;
+        if (MODE != GATED_SUM && b_kfast) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) rb[i] = ((wb[i & 1].rows >> (i >> 1)) & 1u) && bk < left ? wb[i & 1].at[(i >> 1) * wb[i & 1].step] : 0.0;
+            wb[1].at += wb[1].panel;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) rb[i] = ((wb[0].rows >> i) & 1u) && bk + (b_kfast ? 0 : 2 * i) < left ? wb[0].at[i * wb[0].step] : 0.0;
         }
+        wb[0].at += wb[0].panel;
     };
-    auto stash = [&](int64_t panel, int buf) {
-        const int phase = MODE == GATED_SUM && panel >= phase_panels;
+    auto stash = [&](int buf) {   // (what the last fetch brought, by the same places)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            int r, k;
-            place(p.a[phase].cs == 1, i, &r, &k);
-            As[buf][0][r][k] = ra[i];
-            place(p.b[phase].rs == 1, i, &r, &k);
-            As[buf][1][r][k] = rb[i];
+            As[buf][0][a_kfast ? (tid >> 4) + 8 * i : tid & 63][a_kfast ? tid & 15 : (tid >> 6) + 2 * i] = ra[i];
+            As[buf][1][b_kfast ? (tid >> 4) + 8 * i : tid & 63][b_kfast ? tid & 15 : (tid >> 6) + 2 * i] = rb[i];
         }
     };
     double acc[4][4][2];
@@ -159,7 +190,7 @@ __global__ void __launch_bounds__(128, 3) nk_gated_dmma_kernel(const GatedTile p
     const int wm = (warp >> 1) * 32, wn = (warp & 1) * 32, fr = lane >> 2, fk = lane & 3;
     if (first < last) {
         fetch(first);
-        stash(first, 0);
+        stash(0);
     }
     __syncthreads();
     int buf = 0;
@@ -179,7 +210,7 @@ __global__ void __launch_bounds__(128, 3) nk_gated_dmma_kernel(const GatedTile p
                 for (int j = 0; j < 4; j++) gd_mma(acc[i][j], a[i], b[j]);
         }
         if (more) {
-            stash(panel + 1, buf ^ 1);   // the other buffer was last read one panel ago, before the barrier below
+            stash(buf ^ 1);   // the other buffer was last read one panel ago, before the barrier below
             __syncthreads();
             buf ^= 1;
         }
