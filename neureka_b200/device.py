@@ -17,6 +17,7 @@ import numpy as np
 
 from . import _lib as L
 from .ndconf import NDConfiguration
+from .tensor import Tensor
 
 NP_TO_NK = {
     np.dtype(np.float32): L.NK_F32, np.dtype(np.float64): L.NK_F64, np.dtype(np.int8): L.NK_I8,
@@ -40,7 +41,7 @@ class CudaData:
         self.size = int(size)
         self.dtype = np.dtype(dtype)
         self.usages = 0
-        self._finalizer = weakref.finalize(self, CudaDevice._release, device, buf)
+        self.alive = True
 
     def increment_usage(self) -> None:
         self.usages += 1
@@ -51,12 +52,15 @@ class CudaData:
             self.free()
 
     def free(self) -> None:
-        if self._finalizer.alive:
-            self._finalizer()
+        if self.alive:
+            self.alive = False
+            CudaDevice._release(self.device, self.buf)
 
-    @property
-    def alive(self) -> bool:
-        return self._finalizer.alive
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:   # interpreter shutdown: the library may already be gone
+            pass
 
 
 class Access:
@@ -172,9 +176,9 @@ class CudaDevice:
 
     # ---- raw allocation ------------------------------------------------------------------------------
     @staticmethod
-    def _release(device: "CudaDevice", buf: int) -> None:
+    def _release(device: "CudaDevice", buf: C.c_void_p) -> None:
         if device.ctx is not None:
-            L.lib.nk_free(device.ctx, C.c_void_p(buf))
+            L.lib.nk_free(device.ctx, buf)
             device._n_data -= 1
 
     def _alloc(self, dtype, size: int) -> CudaData:
@@ -206,9 +210,8 @@ class CudaDevice:
 
     def new_tensor(self, dtype, shape):
         """A tensor of this shape on the device whose elements hold nothing yet: for drains a kernel writes completely."""
-        from .tensor import Tensor
         t = Tensor(dtype, NDConfiguration.of_shape(shape), None)
-        t._attach(self._alloc(t.dtype, t.size), self)
+        t._attach(self._alloc(t.dtype, t.ndconf.size), self)
         self._stored.add(t)
         return t
 
@@ -268,7 +271,7 @@ class CudaDevice:
 
     def has(self, tensor) -> bool:
         data = tensor._data
-        return isinstance(data, CudaData) and data.device is self and tensor in self._stored
+        return isinstance(data, CudaData) and data.device is self and tensor.device is self
 
     contains = has
 
@@ -288,8 +291,9 @@ class CudaDevice:
 
     def approve(self, call) -> "CudaDevice":
         """Device.approve (Device.java:195): all inputs must live here and share a supported type."""
+        has = self.has
         for t in call.inputs:
-            if t is not None and not self.has(t):
+            if t is not None and not has(t):
                 raise ValueError("every input of a call must be stored on the executing device")
         return self
 

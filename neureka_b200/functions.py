@@ -193,12 +193,11 @@ def _execute_on_common_device(call: ExecutionCall, impl) -> Tensor:
     """AbstractDeviceAlgorithm.executeOnCommonDevice (:427-449) + executeDeviceAlgorithm (:127-156)."""
     dev = call.device
     moved = []
-    for t in call.inputs:   # AbstractDeviceAlgorithm.java:119-124, :130-134
-        if t is None:
-            raise ValueError("Device arguments may not be null!\n"
-                             "One or more tensor arguments within the given ExecutionCall instance is null.")
+    if None in call.inputs:   # AbstractDeviceAlgorithm.java:119-124, :130-134
+        raise ValueError("Device arguments may not be null!\n"
+                         "One or more tensor arguments within the given ExecutionCall instance is null.")
     for t in call.inputs:
-        if t is not None and not dev.has(t):
+        if not dev.has(t):
             dev.store(t)
             moved.append(t)
     dev.approve(call)

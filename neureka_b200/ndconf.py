@@ -72,12 +72,12 @@ class NDConfiguration:
     @staticmethod
     def of_shape(shape, layout: Layout = Layout.ROW_MAJOR) -> "NDConfiguration":
         """The configuration of a freshly created tensor (NDConstructor: row-major strides and indicesMap)."""
-        return _of_shape(tuple(int(x) for x in shape), layout)
+        return _of_shape(shape if type(shape) is tuple else tuple(shape), layout)
 
     @staticmethod
     def virtual_of(shape) -> "NDConfiguration":
         """VirtualNDConfiguration (ndim/config/types/views/virtual/VirtualNDConfiguration.java): one element stands for all."""
-        return _virtual_of(tuple(int(x) for x in shape))
+        return _virtual_of(shape if type(shape) is tuple else tuple(shape))
 
     # ---- queries (a configuration never changes: what is asked for with every call is worked out once) -----
     @cached_property
@@ -102,6 +102,10 @@ class NDConfiguration:
 
     def is_compact(self) -> bool:
         """isCompact (NDConfiguration.java:386-392)."""
+        return self._compact
+
+    @cached_property
+    def _compact(self) -> bool:
         return all(s in (0, 1) for s in self.spread) and all(o == 0 for o in self.offset)
 
     def layout(self) -> Layout:
@@ -187,6 +191,7 @@ class NDConfiguration:
 # A program makes tensors of the same few shapes over and over: their (immutable) configurations are shared.
 @lru_cache(maxsize=4096)
 def _of_shape(shape: Tuple[int, ...], layout: Layout) -> NDConfiguration:
+    shape = tuple(int(x) for x in shape)
     rm = Layout.ROW_MAJOR.new_strides_for(shape)
     strides = layout.new_strides_for(shape) if layout is Layout.COLUMN_MAJOR else rm
     n = len(shape)
@@ -195,5 +200,6 @@ def _of_shape(shape: Tuple[int, ...], layout: Layout) -> NDConfiguration:
 
 @lru_cache(maxsize=4096)
 def _virtual_of(shape: Tuple[int, ...]) -> NDConfiguration:
+    shape = tuple(int(x) for x in shape)
     z = (0,) * len(shape)
     return NDConfiguration(shape, z, z, z, z, True)
