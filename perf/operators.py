@@ -215,17 +215,17 @@ def _tensor(device, values):
     return t
 
 
+class _Pointer:
+    """what a view of a tensor's memory holds on to"""
+
+
 def _as_torch(tensor):
     """a tensor's memory as torch sees it (no copy); keeps the tensor alive"""
     import ctypes as C
     from neureka_b200 import _lib as L
-
-    class Pointer:
-        pass
-
     ptr = C.c_void_p()
     L.check(L.lib.nk_buf_info(tensor._data.buf, C.byref(ptr), None, None))
-    at = Pointer()
+    at = _Pointer()
     at.tensor = tensor
     at.__cuda_array_interface__ = {"shape": tensor.shape, "typestr": "<f4" if tensor.dtype == np.float32 else "<f8", "data": (ptr.value, False), "version": 3}
     return torch.as_tensor(at, device="cuda")
