@@ -8,6 +8,7 @@
 #include <cooperative_groups.h>
 
 #include "nk_internal.h"
+#include "nk_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -26,6 +27,7 @@ struct NormPlan {
     int64_t s[3][NK_MAX_RANK], inner[3];     // 0: drain, 1: source, 2: error; strides of the outer dims and of the normalised one
     int64_t gain_s, shift_s;                 // strides of gain and shift
     int gain_v, shift_v;                     // 16-byte loads of them are possible
+    const char *lo[2], *hi[2];               // the buffers of source and error
 };
 
 template <int OP>
@@ -351,6 +353,338 @@ __global__ void __launch_bounds__(256) nk_norm_grad_lanes_kernel(T* out, const T
     for (int64_t c = threadIdx.x; c < p.n; c += 256) { part[c] = sums[0][c]; part[p.n + c] = sums[1][c]; }
 }
 
+// ---- many rows: one CTA per SM, rows fetched ahead by bulk copies --------------------------------------------------------------------
+// A team of TW warps takes a row at a time. Its rows arrive in shared memory by cp.async.bulk, several ahead, so that the memory is kept busy
+// through the reductions; the copies need nothing but 16-byte boundaries around a row, so rows that start anywhere cost no more than aligned ones
+// (element-wise loads of rows into registers reached a third of the memory's rate). A row's 16-byte boundaries may lie outside its buffer at
+// the buffer's ends: such a row is read by plain loads.
+constexpr int STREAM_WARPS = 16, STREAM_THREADS = 512, STREAM_SMEM = 200 * 1024, STREAM_STAGES = 8;
+
+__device__ __forceinline__ void norm_bulk_load(void* smem, const void* gmem, unsigned bytes, uint64_t* bar) {
+    const unsigned d = (unsigned)__cvta_generic_to_shared(smem), b = (unsigned)__cvta_generic_to_shared(bar);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(d), "l"(gmem), "r"(bytes), "r"(b) : "memory");
+}
+// a row (or a cluster's CTA's slice of one) of a tensor and the 16-byte blocks around it
+template <class T>
+struct StreamRow {
+    const T* at;
+    const char* from;
+    unsigned bytes;
+    bool inside;   // the blocks lie in the buffer
+    __device__ __forceinline__ StreamRow(const T* row, int64_t cols, const char* lo, const char* hi) {
+        at = row;
+        const uintptr_t a = reinterpret_cast<uintptr_t>(row);
+        from = reinterpret_cast<const char*>(a & ~uintptr_t(15));
+        bytes = unsigned(((a + uintptr_t(cols) * sizeof(T) + 15) & ~uintptr_t(15)) - (a & ~uintptr_t(15)));
+        inside = from >= lo && from + bytes <= hi;
+    }
+    __device__ __forceinline__ int offset() const { return int((reinterpret_cast<const char*>(at) - from) / int(sizeof(T))); }
+};
+struct StreamCall {
+    const char *lo[2], *hi[2];   // the buffers of source and error
+    int stages, stage_bytes;     // of one row
+    int cols;                    // columns of a CTA's slice (n for a CTA alone)
+    int* status;
+};
+
+// sums over a team, the same in every thread; `turn` alternates between the calls' shared memory
+template <class T, int TW, int K>
+__device__ __forceinline__ void team_sum(T (&v)[K], T (*smem)[K], int team) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < K; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if (TW == 1) { __syncwarp(); return; }
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int i = 0; i < K; i++) smem[(threadIdx.x >> 5) % TW][i] = v[i];
+    asm volatile("bar.sync %0, %1;\n" ::"r"(1 + team), "n"(TW * 32) : "memory");
+#pragma unroll
+    for (int i = 0; i < K; i++) {
+        v[i] = smem[0][i];
+#pragma unroll
+        for (int w = 1; w < TW; w++) v[i] += smem[w][i];
+    }
+}
+
+// What both kernels share: the team's ring of rows.
+template <class T, int TW, int TENSORS>
+struct StreamRing {
+    const NormPlan& p;
+    const StreamCall& c;
+    unsigned char* base;
+    uint64_t* bars;
+    const T* src[2];
+    int64_t step, next;   // rows between this team's rows; the next one to be fetched
+    int64_t c0;           // first column of the slice
+    int64_t cols;
+    int slot, fetch_slot;
+    unsigned phase;
+    bool leader, dead;
+
+    __device__ __forceinline__ const T* row_of(int t, int64_t row) const { return src[t] + (t ? norm_row<2>(p, row) : norm_row<1>(p, row)) + c0; }
+    __device__ __forceinline__ unsigned char* stage(int s, int t) const { return base + (size_t(s) * TENSORS + t) * c.stage_bytes; }
+    // requests the next row into the slot that was consumed last
+    __device__ __forceinline__ void fetch() {
+        if (leader && !dead && next < p.rows) {
+            unsigned bytes = 0;
+            bool any = false;
+#pragma unroll
+            for (int t = 0; t < TENSORS; t++) {
+                const StreamRow<T> r(row_of(t, next), cols, c.lo[t], c.hi[t]);
+                if (r.inside) { bytes += r.bytes; any = true; }
+            }
+            if (any) {
+                nk_mbar_expect_tx(&bars[fetch_slot], bytes);
+#pragma unroll
+                for (int t = 0; t < TENSORS; t++) {
+                    const StreamRow<T> r(row_of(t, next), cols, c.lo[t], c.hi[t]);
+                    if (r.inside) norm_bulk_load(stage(fetch_slot, t), r.from, r.bytes, &bars[fetch_slot]);
+                }
+            } else nk_mbar_arrive(&bars[fetch_slot]);
+        }
+        next += step;
+        if (++fetch_slot == c.stages) fetch_slot = 0;
+    }
+    __device__ __forceinline__ void wait() {
+        if (dead) return;
+        if (nk_mbar_wait_bounded(&bars[slot], phase, NK_WAIT_LIMIT_NS, nullptr) < 0) {
+            dead = true;   // nothing more is fetched; what is on its way still lands
+            if (c.status) atomicExch(c.status, 1);
+            for (int i = 1; leader && i < c.stages; i++)
+                if (next - (c.stages - i) * step < p.rows) nk_mbar_wait_bounded(&bars[(slot + i) % c.stages], phase ^ unsigned(slot + i >= c.stages), NK_WAIT_LIMIT_NS, nullptr);
+        }
+    }
+    __device__ __forceinline__ void advance() {
+        if (++slot == c.stages) { slot = 0; phase ^= 1u; }
+    }
+    // where the row of tensor t that is due can be read: shared memory, or (outside) the row itself
+    __device__ __forceinline__ const T* due(int t, int64_t row) const {
+        const StreamRow<T> r(row_of(t, row), cols, c.lo[t], c.hi[t]);
+        return r.inside ? reinterpret_cast<const T*>(stage(slot, t)) + r.offset() : r.at;
+    }
+};
+template <class T, int W>
+__device__ __forceinline__ void stream_read(const T* row, int c, T (&v)[W]) {
+    if (W > 1) *reinterpret_cast<typename NormVec<T, W>::type*>(v) = *reinterpret_cast<const typename NormVec<T, W>::type*>(row + c);
+    else v[0] = row[c];
+}
+template <class T, int TW, int TENSORS>
+__device__ __forceinline__ StreamRing<T, TW, TENSORS> stream_ring(const NormPlan& p, const StreamCall& c, const T* src, const T* err, unsigned char* smem, uint64_t* bars) {
+    constexpr int TEAMS = STREAM_WARPS / TW;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int size = int(cluster.num_blocks()), rank = int(cluster.block_rank()), team = (threadIdx.x >> 5) / TW;
+    if (threadIdx.x < unsigned(TEAMS * STREAM_STAGES)) {
+        nk_mbar_init(&bars[threadIdx.x], 1);
+        nk_fence_barrier_init();
+        nk_fence_proxy_async();
+    }
+    __syncthreads();
+    StreamRing<T, TW, TENSORS> r{p, c};
+    r.base = smem + size_t(team) * c.stages * TENSORS * c.stage_bytes;
+    r.bars = bars + team * STREAM_STAGES;
+    r.src[0] = src;
+    r.src[1] = err;
+    r.step = int64_t(gridDim.x / unsigned(size)) * TEAMS;
+    r.next = int64_t(blockIdx.x / unsigned(size)) * TEAMS + team;
+    r.c0 = int64_t(rank) * c.cols;
+    r.cols = p.n - r.c0 < c.cols ? p.n - r.c0 : c.cols;
+    r.slot = r.fetch_slot = 0;
+    r.phase = 0;
+    r.leader = threadIdx.x % (TW * 32) == 0;
+    r.dead = false;
+    return r;
+}
+
+template <class T, int W, int TW, int E>
+__global__ void __launch_bounds__(STREAM_THREADS, 1) nk_norm_stream_kernel(T* out, const T* src, const T* __restrict__ gain, const T* __restrict__ shift, T* __restrict__ stats,
+                                                                          const NormPlan p, T eps, const StreamCall call) {
+    constexpr int NV = E / W, TEAMS = STREAM_WARPS / TW, SPAN = TW * 32 * W;
+    extern __shared__ __align__(16) unsigned char stream_smem[];
+    __shared__ uint64_t bars[TEAMS * STREAM_STAGES];
+    __shared__ T sums[2][TEAMS][TW][1], parts[2][2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int size = int(cluster.num_blocks());
+    auto ring = stream_ring<T, TW, 1>(p, call, src, static_cast<const T*>(nullptr), stream_smem, bars);
+    const int team = (threadIdx.x >> 5) / TW, c_lane = int(threadIdx.x % (TW * 32)) * W, cols = int(ring.cols);
+    const T n = T(p.n);
+    T gv[NV][W], sv[NV][W];
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            const int c = c_lane + k * SPAN + j;
+            gv[k][j] = gain && c < cols ? gain[(ring.c0 + c) * p.gain_s] : T(1);
+            sv[k][j] = shift && c < cols ? shift[(ring.c0 + c) * p.shift_s] : T(0);
+        }
+    int64_t row = ring.next;
+    for (int s = 0; s < call.stages; s++) ring.fetch();
+    int turn = 0;
+    auto total = [&](T v, int which) {
+        T a[1] = {v};
+        team_sum<T, TW, 1>(a, sums[which][team], team);
+        if (size == 1) return a[0];
+        if (threadIdx.x == 0) parts[turn & 1][which] = a[0];
+        cluster.sync();
+        T all = T(0);
+        for (int r = 0; r < size; r++) all += *cluster.map_shared_rank(&parts[turn & 1][which], r);
+        return all;
+    };
+    for (; row < p.rows; row += ring.step, turn++) {
+        ring.wait();
+        const T* x = ring.due(0, row);
+        T v[NV][W], sum = T(0);
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+            if (k * SPAN < cols) {
+                const int c = c_lane + k * SPAN;
+                if (c < cols) stream_read<T, W>(x, c, v[k]);
+                else {
+#pragma unroll
+                    for (int j = 0; j < W; j++) v[k][j] = T(0);
+                }
+#pragma unroll
+                for (int j = 0; j < W; j++) sum += v[k][j];
+            }
+        const T mean = total(sum, 0) / n;   // (a barrier of the team: the row has been read)
+        ring.fetch();
+        ring.advance();
+        T m2 = T(0);
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+            if (k * SPAN < cols) {
+#pragma unroll
+                for (int j = 0; j < W; j++)
+                    if (c_lane + k * SPAN + j < cols) m2 += (v[k][j] - mean) * (v[k][j] - mean);
+            }
+        const T rstd = T(1) / sqrt(total(m2, 1) / n + eps);
+        if (stats && ring.c0 == 0 && ring.leader) { stats[row] = mean; stats[p.rows + row] = rstd; }
+        T* y = out + norm_row<0>(p, row) + ring.c0;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int c = c_lane + k * SPAN;
+            if (c < cols) {
+#pragma unroll
+                for (int j = 0; j < W; j++) v[k][j] = (v[k][j] - mean) * rstd * gv[k][j] + sv[k][j];
+                norm_store<T, W>(y, c, 1, cols, v[k]);
+            }
+        }
+    }
+    if (size > 1) cluster.sync();   // nobody leaves while its sums may still be read
+}
+
+template <class T, int W, int TW, int E>
+__global__ void __launch_bounds__(STREAM_THREADS, 1) nk_norm_grad_stream_kernel(T* out, const T* err, const T* src, const T* __restrict__ gain, const T* __restrict__ stats,
+                                                                               T* __restrict__ cols_out, const NormPlan p, const StreamCall call) {
+    constexpr int NV = E / W, TEAMS = STREAM_WARPS / TW, SPAN = TW * 32 * W;
+    extern __shared__ __align__(16) unsigned char stream_smem[];
+    __shared__ uint64_t bars[TEAMS * STREAM_STAGES];
+    __shared__ T sums[2][TEAMS][TW][2], parts[2][2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int size = int(cluster.num_blocks());
+    auto ring = stream_ring<T, TW, 2>(p, call, src, err, stream_smem, bars);
+    const int team = (threadIdx.x >> 5) / TW, c_lane = int(threadIdx.x % (TW * 32)) * W, cols = int(ring.cols);
+    const T n = T(p.n);
+    T gv[NV][W], sg[NV][W], ss[NV][W];
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            const int c = c_lane + k * SPAN + j;
+            gv[k][j] = gain && c < cols ? gain[(ring.c0 + c) * p.gain_s] : T(1);
+            sg[k][j] = ss[k][j] = T(0);
+        }
+    int64_t row = ring.next;
+    for (int s = 0; s < call.stages; s++) ring.fetch();
+    T mean = T(0), rstd = T(0);
+    if (row < p.rows) { mean = stats[row]; rstd = stats[p.rows + row]; }
+    int turn = 0;
+    for (; row < p.rows; row += ring.step, turn++) {
+        T next_mean = T(0), next_rstd = T(0);   // of the row after: on their way during this one
+        if (row + ring.step < p.rows) { next_mean = stats[row + ring.step]; next_rstd = stats[p.rows + row + ring.step]; }
+        ring.wait();
+        const T *x = ring.due(0, row), *e = ring.due(1, row);
+        T xh[NV][W], g[NV][W], s[2] = {T(0), T(0)};
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int c = c_lane + k * SPAN;
+            if (c < cols) {
+                T ev[W];
+                stream_read<T, W>(x, c, xh[k]);
+                stream_read<T, W>(e, c, ev);
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    xh[k][j] = (xh[k][j] - mean) * rstd;
+                    sg[k][j] += ev[j] * xh[k][j];
+                    ss[k][j] += ev[j];
+                    g[k][j] = ev[j] * gv[k][j];
+                    s[0] += g[k][j];
+                    s[1] += g[k][j] * xh[k][j];
+                }
+            }
+        }
+        team_sum<T, TW, 2>(s, sums[turn & 1][team], team);   // (a barrier of the team: the row has been read)
+        ring.fetch();
+        ring.advance();
+        if (size > 1) {
+            if (threadIdx.x == 0) { parts[turn & 1][0] = s[0]; parts[turn & 1][1] = s[1]; }
+            cluster.sync();
+            s[0] = s[1] = T(0);
+            for (int r = 0; r < size; r++) {
+                const T* theirs = cluster.map_shared_rank(&parts[turn & 1][0], r);
+                s[0] += theirs[0];
+                s[1] += theirs[1];
+            }
+        }
+        if (out) {
+            const T m1 = s[0] / n, m2 = s[1] / n;
+            T* o = out + norm_row<0>(p, row) + ring.c0;
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int c = c_lane + k * SPAN;
+                if (c < cols) {
+#pragma unroll
+                    for (int j = 0; j < W; j++) g[k][j] = rstd * (g[k][j] - m1 - xh[k][j] * m2);
+                    norm_store<T, W>(o, c, 1, cols, g[k]);
+                }
+            }
+        }
+        mean = next_mean;
+        rstd = next_rstd;
+    }
+    if (size > 1) cluster.sync();   // nobody leaves while its sums may still be read
+    if (!cols_out) return;
+    // the teams' column sums, one after the other (all rows have been read: the ring's memory is free)
+    T* all = reinterpret_cast<T*>(stream_smem);
+    if (TEAMS > 1) {
+        for (int t = 0; t < TEAMS; t++) {
+            __syncthreads();
+            if (team != t) continue;
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int j = 0; j < W; j++) {
+                    const int c = c_lane + k * SPAN + j;
+                    if (c >= cols) continue;
+                    all[c] = t ? all[c] + sg[k][j] : sg[k][j];
+                    all[cols + c] = t ? all[cols + c] + ss[k][j] : ss[k][j];
+                }
+        }
+        __syncthreads();
+    }
+    T* part = cols_out + int64_t(blockIdx.x / unsigned(size)) * 2 * p.n + ring.c0;
+    if (TEAMS > 1) {
+        for (int c = threadIdx.x; c < cols; c += STREAM_THREADS) { part[c] = all[c]; part[p.n + c] = all[cols + c]; }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int c = c_lane + k * SPAN;
+            norm_store<T, W>(part, c, 1, cols, sg[k]);
+            norm_store<T, W>(part + p.n, c, 1, cols, ss[k]);
+        }
+    }
+}
+
 // ---- rows of any length: cut into chunks of NORM_THREADS * W * 8 elements, a CTA per chunk ---------------------------------------
 constexpr int NORM_NV = 8;
 
@@ -574,6 +908,70 @@ int norm_launch(nk_ctx* ctx, const char* name, void (*kern)(A...), int64_t rows,
 // elements that a thread of the CTA kernels holds at most, and the longest row that they take (a cluster of eight)
 template <class T> constexpr int norm_e() { return 128 / int(sizeof(T)); }
 
+// Rows by bulk copies: enough of them that every team has some, rows that run along memory. Returns the warps of a team, 0: not this way.
+// (300 rows per SM and less, or up to 256 elements: the kernels above are as fast.)
+template <class T> constexpr int stream_e() { return 64 / int(sizeof(T)); }
+struct StreamShape {
+    int team, cluster, stages, stage_bytes, cols, grid;
+    size_t smem;
+};
+template <class T>
+bool stream_shape(const nk_ctx* ctx, const NormPlan& p, int tensors, StreamShape* s) {
+    constexpr int E = stream_e<T>();
+    if (p.n <= 256 || p.inner[1] != 1 || (tensors == 2 && p.inner[2] != 1) || p.inner[0] != 1 || !p.lo[0]) return false;
+    s->team = 1;
+    while (s->team < STREAM_WARPS && int64_t(s->team) * 32 * E < p.n) s->team *= 2;
+    s->cluster = 1;
+    while (s->cluster < 8 && int64_t(s->cluster) * s->team * 32 * E < p.n) s->cluster *= 2;
+    if (int64_t(s->cluster) * s->team * 32 * E < p.n) return false;
+    s->cols = s->cluster > 1 ? int(((p.n + s->cluster - 1) / s->cluster + 3) / 4 * 4) : int(p.n);   // even slices, on 16-byte boundaries of an aligned row
+    const int sms = ctx->prop.multiProcessorCount, teams = STREAM_WARPS / s->team;
+    s->grid = sms / s->cluster * s->cluster;
+    if (p.rows < int64_t(s->grid / s->cluster) * teams * 2) return false;
+    s->stage_bytes = int((size_t(s->cols) * sizeof(T) + 30) / 16 * 16);
+    s->stages = int(STREAM_SMEM / (size_t(teams) * tensors * s->stage_bytes));
+    if (s->stages > STREAM_STAGES) s->stages = STREAM_STAGES;
+    s->smem = size_t(teams) * s->stages * tensors * s->stage_bytes;
+    return s->stages >= 2;
+}
+template <class... A>
+int stream_launch(nk_ctx* ctx, const char* name, void (*kern)(A...), const StreamShape& s, A... args) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SMEM);
+    if (e != cudaSuccess) return nk_cuda_fail(ctx, e, name);
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(unsigned(s.grid));
+    cfg.blockDim = dim3(STREAM_THREADS);
+    cfg.dynamicSmemBytes = s.smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(s.cluster);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = s.cluster > 1 ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e != cudaSuccess) return nk_cuda_fail(ctx, e, name);
+    return nk_after_launch(ctx, name);
+}
+StreamCall stream_call(const nk_ctx* ctx, const NormPlan& p, const StreamShape& s) {
+    StreamCall c;
+    for (int t = 0; t < 2; t++) { c.lo[t] = p.lo[t]; c.hi[t] = p.hi[t]; }
+    c.stages = s.stages;
+    c.stage_bytes = s.stage_bytes;
+    c.cols = s.cols;
+    c.status = ctx->tma_status_dev;
+    return c;
+}
+template <class T, int W>
+int forward_stream(nk_ctx* ctx, const StreamShape& s, T* out, const T* src, const T* gain, const T* shift, T* stats, const NormPlan& p, T eps) {
+    constexpr int E = stream_e<T>();
+    const StreamCall c = stream_call(ctx, p, s);
+#define NK_TEAM(TW) case TW: return stream_launch(ctx, "nk_norm_stream_kernel", nk_norm_stream_kernel<T, W, TW, E>, s, out, src, gain, shift, stats, p, eps, c)
+    switch (s.team) { NK_TEAM(1); NK_TEAM(2); NK_TEAM(4); NK_TEAM(8); default: NK_TEAM(16); }
+#undef NK_TEAM
+}
+
 template <class T, int W>
 int forward_rows(nk_ctx* ctx, T* out, const T* src, const T* gain, const T* shift, T* stats, const NormPlan& p, T eps) {
     constexpr int E = norm_e<T>();
@@ -596,6 +994,8 @@ int forward_rows(nk_ctx* ctx, T* out, const T* src, const T* gain, const T* shif
 
 template <class T, int W>
 int forward_w(nk_ctx* ctx, T* out, const T* src, const T* gain, const T* shift, T* stats, const NormPlan& p, T eps) {
+    StreamShape shape;
+    if (stream_shape<T>(ctx, p, 1, &shape)) return forward_stream<T, W>(ctx, shape, out, src, gain, shift, stats, p, eps);
     if (p.n <= 4096 * norm_e<T>()) return forward_rows<T, W>(ctx, out, src, gain, shift, stats, p, eps);
     constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
     const int64_t chunks = (p.n + L - 1) / L;
@@ -677,7 +1077,26 @@ int backward_rows(nk_ctx* ctx, const NormGrad<T>& a, const NormPlan& p) {
 }
 
 template <class T, int W>
+int backward_stream(nk_ctx* ctx, const StreamShape& s, const NormGrad<T>& a, const NormPlan& p) {
+    constexpr int E = stream_e<T>();
+    const StreamCall c = stream_call(ctx, p, s);
+    const bool cols = a.dgain || a.dshift;
+    const int64_t groups = s.grid / s.cluster;
+    NkWorkspace ws(ctx);
+    int st;
+    if (cols && (st = ws.get(size_t(groups) * 2 * p.n * sizeof(T)))) return st;
+    T* part = static_cast<T*>(ws.ptr);
+#define NK_TEAM(TW) case TW: st = stream_launch(ctx, "nk_norm_grad_stream_kernel", nk_norm_grad_stream_kernel<T, W, TW, E>, s, a.out, a.err, a.src, a.gain, a.stats, part, p, c); break
+    switch (s.team) { NK_TEAM(1); NK_TEAM(2); NK_TEAM(4); NK_TEAM(8); default: NK_TEAM(16); }
+#undef NK_TEAM
+    if (st || !cols) return st;
+    return columns_finish(ctx, a, static_cast<const T*>(part), p.n, groups);
+}
+
+template <class T, int W>
 int backward_w(nk_ctx* ctx, const NormGrad<T>& a, const NormPlan& p) {
+    StreamShape shape;
+    if (stream_shape<T>(ctx, p, 2, &shape)) return backward_stream<T, W>(ctx, shape, a, p);
     if (p.n <= 2048 * norm_e<T>()) return backward_rows<T, W>(ctx, a, p);
     constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
     const int64_t chunks = (p.n + L - 1) / L, blocks_c = (p.n + NORM_THREADS * W - 1) / (NORM_THREADS * W);
@@ -731,6 +1150,10 @@ int norm_stats(nk_ctx* ctx, const char* who, const nk_buf* stats, int32_t dtype,
     if (stats->n_elems / 2 < rows) return nk_fail(ctx, NK_ERR_BOUNDS, "%s: the statistics need 2 * %lld elements, the buffer holds %lld", who, (long long)rows, (long long)stats->n_elems);
     return NK_OK;
 }
+void norm_bounds(const nk_buf* buf, int t, int32_t dtype, NormPlan* p) {
+    p->lo[t] = static_cast<const char*>(buf->ptr);
+    p->hi[t] = p->lo[t] + buf->n_elems * int64_t(nk_dtype_size(dtype));
+}
 int norm_same_shape(nk_ctx* ctx, const char* who, const NkView& a, const NkView& b) {
     for (int k = 0; k < a.rank; k++)
         if (a.shape[k] != b.shape[k]) return nk_fail(ctx, NK_ERR_BAD_ARG, "%s: shapes differ at dim %d (%lld vs %lld)", who, k, (long long)a.shape[k], (long long)b.shape[k]);
@@ -759,6 +1182,7 @@ extern "C" int nk_layer_norm(nk_ctx* ctx, int32_t dtype, int32_t rank, nk_buf* d
     if ((st = norm_vector(ctx, "nk_layer_norm(gain)", gain, cfg_gain, dtype, p.n, false, &g, &p.gain_s))) return st;
     if ((st = norm_vector(ctx, "nk_layer_norm(shift)", shift, cfg_shift, dtype, p.n, false, &s, &p.shift_s))) return st;
     if (stats && (st = norm_stats(ctx, "nk_layer_norm", stats, dtype, p.rows))) return st;
+    norm_bounds(src, 0, dtype, &p);
     p.gain_v = p.gain_s == 1 && reinterpret_cast<uintptr_t>(g) % 16 == 0;
     p.shift_v = p.shift_s == 1 && reinterpret_cast<uintptr_t>(s) % 16 == 0;
     void* keep = stats ? stats->ptr : nullptr;
@@ -808,6 +1232,8 @@ extern "C" int nk_layer_norm_grad(nk_ctx* ctx, int32_t dtype, int32_t rank, nk_b
     if ((st = norm_vector(ctx, "nk_layer_norm_grad(dshift)", dshift, cfg_dshift, dtype, p.n, true, &ds, &dshift_s))) return st;
     if ((st = norm_stats(ctx, "nk_layer_norm_grad", stats, dtype, p.rows))) return st;
     if (!dsrc && !dg && !ds) return NK_OK;
+    norm_bounds(src, 0, dtype, &p);
+    norm_bounds(err, 1, dtype, &p);
     if (dtype == NK_F32) return norm_grad<float>(ctx, dsrc, v0, dg, dgain_s, ds, dshift_s, err, v2, src, v1, g, stats, p);
     return norm_grad<double>(ctx, dsrc, v0, dg, dgain_s, ds, dshift_s, err, v2, src, v1, g, stats, p);
 }

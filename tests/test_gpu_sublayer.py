@@ -66,6 +66,39 @@ def test_layer_norm_and_its_gradients(device, dtype, shape):
     norm_case(device, np.random.default_rng(sum(shape)), dtype, shape)
 
 
+# enough rows that they are fetched ahead: teams of one to sixteen warps and clusters, rows that start anywhere
+@pytest.mark.parametrize("shape", [(5000, 257), (6000, 300), (2500, 777), (2400, 1024), (1300, 2047), (1200, 2500), (620, 4096), (700, 4097), (400, 8000), (300, 8192), (310, 12001), (160, 16384),
+                                   (90, 30001), (80, 40004)], ids=str)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_norm_of_many_rows(device, dtype, shape):
+    norm_case(device, np.random.default_rng(sum(shape)), dtype, shape)
+    norm_case(device, np.random.default_rng(sum(shape)), dtype, shape, affine=False, view="part")
+
+
+def test_layer_norm_rows_at_the_ends_of_odd_memory(device):
+    """A program's own memory, adopted at an address that is no multiple of 16 and as long as the tensor: nothing outside it is read."""
+    import torch
+    rows, n = 2500, 777
+    rng = np.random.default_rng(9)
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    for shift in (1, 2, 3):
+        memory = torch.full((rows * n + 8,), float("nan"), dtype=torch.float32, device="cuda")
+        memory[shift:shift + rows * n] = torch.from_numpy(x.reshape(-1)).cuda()
+        torch.cuda.synchronize()
+        buf = C.c_void_p()
+        L.check(L.lib.nk_wrap(device.ctx, L.NK_F32, C.c_void_p(memory.data_ptr() + 4 * shift), rows * n, C.byref(buf)), device.ctx)
+        try:
+            out, stats = put(device, np.zeros((rows, n), np.float32)), put(device, np.zeros((2, rows), np.float32))
+            c = out.ndconf.inline_pointer
+            L.check(L.lib.nk_layer_norm(device.ctx, L.NK_F32, 2, out._data.buf, c, buf, c, None, None, None, None, 1e-5, stats._data.buf), device.ctx)
+            want, xh, r = S.norm(x, None, None, 1e-5)
+            S.assert_within(out.numpy(), (want, S.norm_bound(x, None, want, xh, r, S.unit(np.float32))), f"shift {shift}")
+            L.check(L.lib.nk_layer_norm_grad(device.ctx, L.NK_F32, 2, out._data.buf, c, None, None, None, None, buf, c, buf, c, None, None, stats._data.buf), device.ctx)
+            S.assert_within(out.numpy(), S.norm_gradients(x, None, x, 1e-5, S.unit(np.float32))[0], f"dx, shift {shift}")
+        finally:
+            L.lib.nk_free(device.ctx, buf)
+
+
 @pytest.mark.parametrize("view", VIEWS[1:])
 @pytest.mark.parametrize("shape", [(5, 7), (40, 96), (3, 4, 130), (3, 2050), (2, 9000)], ids=str)
 @pytest.mark.parametrize("dtype", TYPES)
@@ -111,7 +144,7 @@ def test_layer_norm_rows_that_are_not_finite_stay_apart(device):
 
 def test_layer_norm_gives_the_same_bits_every_time_and_only_the_gradients_asked_for(device):
     rng = np.random.default_rng(7)
-    for shape in ((1500, 1000), (3, 70000)):
+    for shape in ((1500, 1000), (3, 70000), (2000, 1003)):
         x, e, gain = (rng.standard_normal(s).astype(np.float32) for s in (shape, shape, shape[-1:]))
         got = []
         for wanted in ("xg", "xg", "x", "g"):
