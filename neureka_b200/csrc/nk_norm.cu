@@ -7,6 +7,8 @@
 // comes from the differences to a mean that is known before (no difference of large sums).
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "nk_internal.h"
 #include "nk_ptx.cuh"
 
@@ -364,25 +366,9 @@ __device__ __forceinline__ void norm_bulk_load(void* smem, const void* gmem, uns
     const unsigned d = (unsigned)__cvta_generic_to_shared(smem), b = (unsigned)__cvta_generic_to_shared(bar);
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(d), "l"(gmem), "r"(bytes), "r"(b) : "memory");
 }
-// a row (or a cluster's CTA's slice of one) of a tensor and the 16-byte blocks around it
-template <class T>
-struct StreamRow {
-    const T* at;
-    const char* from;
-    unsigned bytes;
-    bool inside;   // the blocks lie in the buffer
-    __device__ __forceinline__ StreamRow(const T* row, int64_t cols, const char* lo, const char* hi) {
-        at = row;
-        const uintptr_t a = reinterpret_cast<uintptr_t>(row);
-        from = reinterpret_cast<const char*>(a & ~uintptr_t(15));
-        bytes = unsigned(((a + uintptr_t(cols) * sizeof(T) + 15) & ~uintptr_t(15)) - (a & ~uintptr_t(15)));
-        inside = from >= lo && from + bytes <= hi;
-    }
-    __device__ __forceinline__ int offset() const { return int((reinterpret_cast<const char*>(at) - from) / int(sizeof(T))); }
-};
 struct StreamCall {
     const char *lo[2], *hi[2];   // the buffers of source and error
-    int stages, stage_bytes;     // of one row
+    int stages, stage_bytes;     // of the ring; a slot's for one tensor
     int cols;                    // columns of a CTA's slice (n for a CTA alone)
     int* status;
 };
@@ -407,41 +393,43 @@ __device__ __forceinline__ void team_sum(T (&v)[K], T (*smem)[K], int team) {
     }
 }
 
-// What both kernels share: the team's ring of rows.
+// What both kernels share: the team's ring of rows. The leader notes where in its slot a row begins (-1: it was not copied).
 template <class T, int TW, int TENSORS>
 struct StreamRing {
     const NormPlan& p;
     const StreamCall& c;
     unsigned char* base;
     uint64_t* bars;
+    int (*places)[TENSORS];
     const T* src[2];
     int64_t step, next;   // rows between this team's rows; the next one to be fetched
     int64_t c0;           // first column of the slice
-    int64_t cols;
+    int cols;
     int slot, fetch_slot;
     unsigned phase;
     bool leader, dead;
 
     __device__ __forceinline__ const T* row_of(int t, int64_t row) const { return src[t] + (t ? norm_row<2>(p, row) : norm_row<1>(p, row)) + c0; }
-    __device__ __forceinline__ unsigned char* stage(int s, int t) const { return base + (size_t(s) * TENSORS + t) * c.stage_bytes; }
+    __device__ __forceinline__ unsigned char* stage(int s, int t) const { return base + (s * TENSORS + t) * c.stage_bytes; }
     // requests the next row into the slot that was consumed last
     __device__ __forceinline__ void fetch() {
         if (leader && !dead && next < p.rows) {
-            unsigned bytes = 0;
-            bool any = false;
+            unsigned bytes[TENSORS], all = 0;
+            const char* from[TENSORS];
 #pragma unroll
-            for (int t = 0; t < TENSORS; t++) {
-                const StreamRow<T> r(row_of(t, next), cols, c.lo[t], c.hi[t]);
-                if (r.inside) { bytes += r.bytes; any = true; }
+            for (int t = 0; t < TENSORS; t++) {   // the 16-byte blocks around the row, where they lie in its buffer
+                const uintptr_t a = reinterpret_cast<uintptr_t>(row_of(t, next)), lo = a & ~uintptr_t(15), hi = (a + unsigned(cols) * sizeof(T) + 15) & ~uintptr_t(15);
+                const bool inside = reinterpret_cast<const char*>(lo) >= c.lo[t] && reinterpret_cast<const char*>(hi) <= c.hi[t];
+                from[t] = reinterpret_cast<const char*>(lo);
+                bytes[t] = inside ? unsigned(hi - lo) : 0u;
+                all += bytes[t];
+                places[fetch_slot][t] = inside ? int(a - lo) : -1;
             }
-            if (any) {
-                nk_mbar_expect_tx(&bars[fetch_slot], bytes);
+            if (all) nk_mbar_expect_tx(&bars[fetch_slot], all);
+            else nk_mbar_arrive(&bars[fetch_slot]);
 #pragma unroll
-                for (int t = 0; t < TENSORS; t++) {
-                    const StreamRow<T> r(row_of(t, next), cols, c.lo[t], c.hi[t]);
-                    if (r.inside) norm_bulk_load(stage(fetch_slot, t), r.from, r.bytes, &bars[fetch_slot]);
-                }
-            } else nk_mbar_arrive(&bars[fetch_slot]);
+            for (int t = 0; t < TENSORS; t++)
+                if (bytes[t]) norm_bulk_load(stage(fetch_slot, t), from[t], bytes[t], &bars[fetch_slot]);
         }
         next += step;
         if (++fetch_slot == c.stages) fetch_slot = 0;
@@ -458,10 +446,10 @@ struct StreamRing {
     __device__ __forceinline__ void advance() {
         if (++slot == c.stages) { slot = 0; phase ^= 1u; }
     }
-    // where the row of tensor t that is due can be read: shared memory, or (outside) the row itself
+    // where the row of tensor t that is due can be read: shared memory, or (not copied) the row itself
     __device__ __forceinline__ const T* due(int t, int64_t row) const {
-        const StreamRow<T> r(row_of(t, row), cols, c.lo[t], c.hi[t]);
-        return r.inside ? reinterpret_cast<const T*>(stage(slot, t)) + r.offset() : r.at;
+        const int at = places[slot][t];
+        return at >= 0 ? reinterpret_cast<const T*>(stage(slot, t) + at) : row_of(t, row);
     }
 };
 template <class T, int W>
@@ -469,8 +457,14 @@ __device__ __forceinline__ void stream_read(const T* row, int c, T (&v)[W]) {
     if (W > 1) *reinterpret_cast<typename NormVec<T, W>::type*>(v) = *reinterpret_cast<const typename NormVec<T, W>::type*>(row + c);
     else v[0] = row[c];
 }
+template <class T, int W>
+__device__ __forceinline__ void stream_write(T* row, int c, const T (&v)[W]) {
+    if (W > 1) *reinterpret_cast<typename NormVec<T, W>::type*>(row + c) = *reinterpret_cast<const typename NormVec<T, W>::type*>(v);
+    else row[c] = v[0];
+}
 template <class T, int TW, int TENSORS>
-__device__ __forceinline__ StreamRing<T, TW, TENSORS> stream_ring(const NormPlan& p, const StreamCall& c, const T* src, const T* err, unsigned char* smem, uint64_t* bars) {
+__device__ __forceinline__ StreamRing<T, TW, TENSORS> stream_ring(const NormPlan& p, const StreamCall& c, const T* src, const T* err, unsigned char* smem, uint64_t* bars,
+                                                               int (*places)[TENSORS]) {
     constexpr int TEAMS = STREAM_WARPS / TW;
     cg::cluster_group cluster = cg::this_cluster();
     const int size = int(cluster.num_blocks()), rank = int(cluster.block_rank()), team = (threadIdx.x >> 5) / TW;
@@ -483,12 +477,13 @@ __device__ __forceinline__ StreamRing<T, TW, TENSORS> stream_ring(const NormPlan
     StreamRing<T, TW, TENSORS> r{p, c};
     r.base = smem + size_t(team) * c.stages * TENSORS * c.stage_bytes;
     r.bars = bars + team * STREAM_STAGES;
+    r.places = places + team * STREAM_STAGES;
     r.src[0] = src;
     r.src[1] = err;
     r.step = int64_t(gridDim.x / unsigned(size)) * TEAMS;
     r.next = int64_t(blockIdx.x / unsigned(size)) * TEAMS + team;
     r.c0 = int64_t(rank) * c.cols;
-    r.cols = p.n - r.c0 < c.cols ? p.n - r.c0 : c.cols;
+    r.cols = p.n - r.c0 < c.cols ? int(p.n - r.c0) : c.cols;
     r.slot = r.fetch_slot = 0;
     r.phase = 0;
     r.leader = threadIdx.x % (TW * 32) == 0;
@@ -496,78 +491,78 @@ __device__ __forceinline__ StreamRing<T, TW, TENSORS> stream_ring(const NormPlan
     return r;
 }
 
+// A lane's vectors k < mine of a slice, SPAN columns apart. No thread of the team has more than `most`, which is looked at every fourth time (a branch
+// per vector keeps their loads from being in flight together; none costs the instructions of vectors that nobody has).
+#define NK_EACH(k) _Pragma("unroll") for (int k = 0; k < NV; k++) if (k % 4 == 0 && k >= most) break; else if (k < mine)
+
 template <class T, int W, int TW, int E>
 __global__ void __launch_bounds__(STREAM_THREADS, 1) nk_norm_stream_kernel(T* out, const T* src, const T* __restrict__ gain, const T* __restrict__ shift, T* __restrict__ stats,
                                                                           const NormPlan p, T eps, const StreamCall call) {
     constexpr int NV = E / W, TEAMS = STREAM_WARPS / TW, SPAN = TW * 32 * W;
     extern __shared__ __align__(16) unsigned char stream_smem[];
     __shared__ uint64_t bars[TEAMS * STREAM_STAGES];
+    __shared__ int places[TEAMS * STREAM_STAGES][1];
     __shared__ T sums[2][TEAMS][TW][1], parts[2][2];
     cg::cluster_group cluster = cg::this_cluster();
     const int size = int(cluster.num_blocks());
-    auto ring = stream_ring<T, TW, 1>(p, call, src, static_cast<const T*>(nullptr), stream_smem, bars);
-    const int team = (threadIdx.x >> 5) / TW, c_lane = int(threadIdx.x % (TW * 32)) * W, cols = int(ring.cols);
-    const T n = T(p.n);
+    auto ring = stream_ring<T, TW, 1>(p, call, src, static_cast<const T*>(nullptr), stream_smem, bars, places);
+    const int team = (threadIdx.x >> 5) / TW, c_lane = int(threadIdx.x % (TW * 32)) * W, cols = ring.cols;
+    const int most = (cols + SPAN - 1) / SPAN, mine = c_lane < cols ? (cols - c_lane + SPAN - 1) / SPAN : 0;
+    const T inv_n = T(1) / T(p.n), inv_cols = T(1) / T(cols);
     T gv[NV][W], sv[NV][W];
-#pragma unroll
-    for (int k = 0; k < NV; k++)
+    NK_EACH(k) {
 #pragma unroll
         for (int j = 0; j < W; j++) {
-            const int c = c_lane + k * SPAN + j;
-            gv[k][j] = gain && c < cols ? gain[(ring.c0 + c) * p.gain_s] : T(1);
-            sv[k][j] = shift && c < cols ? shift[(ring.c0 + c) * p.shift_s] : T(0);
+            const int64_t c = ring.c0 + c_lane + k * SPAN + j;
+            gv[k][j] = gain ? gain[c * p.gain_s] : T(1);
+            sv[k][j] = shift ? shift[c * p.shift_s] : T(0);
         }
+    }
     int64_t row = ring.next;
     for (int s = 0; s < call.stages; s++) ring.fetch();
-    int turn = 0;
-    auto total = [&](T v, int which) {
-        T a[1] = {v};
-        team_sum<T, TW, 1>(a, sums[which][team], team);
-        if (size == 1) return a[0];
-        if (threadIdx.x == 0) parts[turn & 1][which] = a[0];
-        cluster.sync();
-        T all = T(0);
-        for (int r = 0; r < size; r++) all += *cluster.map_shared_rank(&parts[turn & 1][which], r);
-        return all;
-    };
-    for (; row < p.rows; row += ring.step, turn++) {
+    for (int turn = 0; row < p.rows; row += ring.step, turn++) {
         ring.wait();
-        const T* x = ring.due(0, row);
-        T v[NV][W], sum = T(0);
+        const T* x = ring.due(0, row) + c_lane;
+        T v[NV][W], sum[1] = {T(0)};
+        NK_EACH(k) {
+            stream_read<T, W>(x, k * SPAN, v[k]);
 #pragma unroll
-        for (int k = 0; k < NV; k++)
-            if (k * SPAN < cols) {
-                const int c = c_lane + k * SPAN;
-                if (c < cols) stream_read<T, W>(x, c, v[k]);
-                else {
-#pragma unroll
-                    for (int j = 0; j < W; j++) v[k][j] = T(0);
-                }
-#pragma unroll
-                for (int j = 0; j < W; j++) sum += v[k][j];
-            }
-        const T mean = total(sum, 0) / n;   // (a barrier of the team: the row has been read)
+            for (int j = 0; j < W; j++) sum[0] += v[k][j];
+        }
+        team_sum<T, TW, 1>(sum, sums[0][team], team);   // (a barrier of the team: the row has been read)
         ring.fetch();
         ring.advance();
-        T m2 = T(0);
+        T mean = sum[0] * inv_cols, m2[1] = {T(0)};
+        NK_EACH(k) {
 #pragma unroll
-        for (int k = 0; k < NV; k++)
-            if (k * SPAN < cols) {
-#pragma unroll
-                for (int j = 0; j < W; j++)
-                    if (c_lane + k * SPAN + j < cols) m2 += (v[k][j] - mean) * (v[k][j] - mean);
+            for (int j = 0; j < W; j++) m2[0] += (v[k][j] - mean) * (v[k][j] - mean);
+        }
+        team_sum<T, TW, 1>(m2, sums[1][team], team);
+        if (size > 1) {   // the slices' means and squares: mu = sum(n_i mu_i) / n, v = sum(m2_i + n_i (mu_i - mu)^2) / n
+            if (threadIdx.x == 0) { parts[turn & 1][0] = mean; parts[turn & 1][1] = m2[0]; }
+            cluster.sync();
+            T all = T(0), all2 = T(0);
+            for (int r = 0; r < size; r++) {
+                const int64_t left = p.n - int64_t(r) * call.cols;
+                all += T(left < call.cols ? left : call.cols) * cluster.map_shared_rank(&parts[turn & 1][0], r)[0];
             }
-        const T rstd = T(1) / sqrt(total(m2, 1) / n + eps);
+            all *= inv_n;
+            for (int r = 0; r < size; r++) {
+                const int64_t left = p.n - int64_t(r) * call.cols;
+                const T* theirs = cluster.map_shared_rank(&parts[turn & 1][0], r);
+                const T d = theirs[0] - all;
+                all2 += theirs[1] + T(left < call.cols ? left : call.cols) * d * d;
+            }
+            mean = all;
+            m2[0] = all2;
+        }
+        const T rstd = T(1) / sqrt(m2[0] * inv_n + eps);
         if (stats && ring.c0 == 0 && ring.leader) { stats[row] = mean; stats[p.rows + row] = rstd; }
-        T* y = out + norm_row<0>(p, row) + ring.c0;
+        T* y = out + norm_row<0>(p, row) + ring.c0 + c_lane;
+        NK_EACH(k) {
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int c = c_lane + k * SPAN;
-            if (c < cols) {
-#pragma unroll
-                for (int j = 0; j < W; j++) v[k][j] = (v[k][j] - mean) * rstd * gv[k][j] + sv[k][j];
-                norm_store<T, W>(y, c, 1, cols, v[k]);
-            }
+            for (int j = 0; j < W; j++) v[k][j] = (v[k][j] - mean) * rstd * gv[k][j] + sv[k][j];
+            stream_write<T, W>(y, k * SPAN, v[k]);
         }
     }
     if (size > 1) cluster.sync();   // nobody leaves while its sums may still be read
@@ -579,48 +574,44 @@ __global__ void __launch_bounds__(STREAM_THREADS, 1) nk_norm_grad_stream_kernel(
     constexpr int NV = E / W, TEAMS = STREAM_WARPS / TW, SPAN = TW * 32 * W;
     extern __shared__ __align__(16) unsigned char stream_smem[];
     __shared__ uint64_t bars[TEAMS * STREAM_STAGES];
+    __shared__ int places[TEAMS * STREAM_STAGES][2];
     __shared__ T sums[2][TEAMS][TW][2], parts[2][2];
     cg::cluster_group cluster = cg::this_cluster();
     const int size = int(cluster.num_blocks());
-    auto ring = stream_ring<T, TW, 2>(p, call, src, err, stream_smem, bars);
-    const int team = (threadIdx.x >> 5) / TW, c_lane = int(threadIdx.x % (TW * 32)) * W, cols = int(ring.cols);
-    const T n = T(p.n);
+    auto ring = stream_ring<T, TW, 2>(p, call, src, err, stream_smem, bars, places);
+    const int team = (threadIdx.x >> 5) / TW, c_lane = int(threadIdx.x % (TW * 32)) * W, cols = ring.cols;
+    const int most = (cols + SPAN - 1) / SPAN, mine = c_lane < cols ? (cols - c_lane + SPAN - 1) / SPAN : 0;
+    const T inv_n = T(1) / T(p.n);
     T gv[NV][W], sg[NV][W], ss[NV][W];
 #pragma unroll
     for (int k = 0; k < NV; k++)
 #pragma unroll
         for (int j = 0; j < W; j++) {
-            const int c = c_lane + k * SPAN + j;
-            gv[k][j] = gain && c < cols ? gain[(ring.c0 + c) * p.gain_s] : T(1);
+            gv[k][j] = gain && k < mine ? gain[(ring.c0 + c_lane + k * SPAN + j) * p.gain_s] : T(1);
             sg[k][j] = ss[k][j] = T(0);
         }
     int64_t row = ring.next;
     for (int s = 0; s < call.stages; s++) ring.fetch();
     T mean = T(0), rstd = T(0);
     if (row < p.rows) { mean = stats[row]; rstd = stats[p.rows + row]; }
-    int turn = 0;
-    for (; row < p.rows; row += ring.step, turn++) {
+    for (int turn = 0; row < p.rows; row += ring.step, turn++) {
         T next_mean = T(0), next_rstd = T(0);   // of the row after: on their way during this one
         if (row + ring.step < p.rows) { next_mean = stats[row + ring.step]; next_rstd = stats[p.rows + row + ring.step]; }
         ring.wait();
-        const T *x = ring.due(0, row), *e = ring.due(1, row);
+        const T *x = ring.due(0, row) + c_lane, *e = ring.due(1, row) + c_lane;
         T xh[NV][W], g[NV][W], s[2] = {T(0), T(0)};
+        NK_EACH(k) {
+            T ev[W];
+            stream_read<T, W>(x, k * SPAN, xh[k]);
+            stream_read<T, W>(e, k * SPAN, ev);
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int c = c_lane + k * SPAN;
-            if (c < cols) {
-                T ev[W];
-                stream_read<T, W>(x, c, xh[k]);
-                stream_read<T, W>(e, c, ev);
-#pragma unroll
-                for (int j = 0; j < W; j++) {
-                    xh[k][j] = (xh[k][j] - mean) * rstd;
-                    sg[k][j] += ev[j] * xh[k][j];
-                    ss[k][j] += ev[j];
-                    g[k][j] = ev[j] * gv[k][j];
-                    s[0] += g[k][j];
-                    s[1] += g[k][j] * xh[k][j];
-                }
+            for (int j = 0; j < W; j++) {
+                xh[k][j] = (xh[k][j] - mean) * rstd;
+                sg[k][j] += ev[j] * xh[k][j];
+                ss[k][j] += ev[j];
+                g[k][j] = ev[j] * gv[k][j];
+                s[0] += g[k][j];
+                s[1] += g[k][j] * xh[k][j];
             }
         }
         team_sum<T, TW, 2>(s, sums[turn & 1][team], team);   // (a barrier of the team: the row has been read)
@@ -637,16 +628,12 @@ __global__ void __launch_bounds__(STREAM_THREADS, 1) nk_norm_grad_stream_kernel(
             }
         }
         if (out) {
-            const T m1 = s[0] / n, m2 = s[1] / n;
-            T* o = out + norm_row<0>(p, row) + ring.c0;
+            const T m1 = s[0] * inv_n, m2 = s[1] * inv_n;
+            T* o = out + norm_row<0>(p, row) + ring.c0 + c_lane;
+            NK_EACH(k) {
 #pragma unroll
-            for (int k = 0; k < NV; k++) {
-                const int c = c_lane + k * SPAN;
-                if (c < cols) {
-#pragma unroll
-                    for (int j = 0; j < W; j++) g[k][j] = rstd * (g[k][j] - m1 - xh[k][j] * m2);
-                    norm_store<T, W>(o, c, 1, cols, g[k]);
-                }
+                for (int j = 0; j < W; j++) g[k][j] = rstd * (g[k][j] - m1 - xh[k][j] * m2);
+                stream_write<T, W>(o, k * SPAN, g[k]);
             }
         }
         mean = next_mean;
@@ -654,36 +641,32 @@ __global__ void __launch_bounds__(STREAM_THREADS, 1) nk_norm_grad_stream_kernel(
     }
     if (size > 1) cluster.sync();   // nobody leaves while its sums may still be read
     if (!cols_out) return;
+    T* part = cols_out + int64_t(blockIdx.x / unsigned(size)) * 2 * p.n + ring.c0;
+    if (TEAMS == 1) {
+        NK_EACH(k) {
+            stream_write<T, W>(part + c_lane, k * SPAN, sg[k]);
+            stream_write<T, W>(part + p.n + c_lane, k * SPAN, ss[k]);
+        }
+        return;
+    }
     // the teams' column sums, one after the other (all rows have been read: the ring's memory is free)
     T* all = reinterpret_cast<T*>(stream_smem);
-    if (TEAMS > 1) {
-        for (int t = 0; t < TEAMS; t++) {
-            __syncthreads();
-            if (team != t) continue;
-#pragma unroll
-            for (int k = 0; k < NV; k++)
-#pragma unroll
-                for (int j = 0; j < W; j++) {
-                    const int c = c_lane + k * SPAN + j;
-                    if (c >= cols) continue;
-                    all[c] = t ? all[c] + sg[k][j] : sg[k][j];
-                    all[cols + c] = t ? all[cols + c] + ss[k][j] : ss[k][j];
-                }
-        }
+    for (int t = 0; t < TEAMS; t++) {
         __syncthreads();
-    }
-    T* part = cols_out + int64_t(blockIdx.x / unsigned(size)) * 2 * p.n + ring.c0;
-    if (TEAMS > 1) {
-        for (int c = threadIdx.x; c < cols; c += STREAM_THREADS) { part[c] = all[c]; part[p.n + c] = all[cols + c]; }
-    } else {
+        if (team != t) continue;
+        NK_EACH(k) {
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int c = c_lane + k * SPAN;
-            norm_store<T, W>(part, c, 1, cols, sg[k]);
-            norm_store<T, W>(part + p.n, c, 1, cols, ss[k]);
+            for (int j = 0; j < W; j++) {
+                const int c = c_lane + k * SPAN + j;
+                all[c] = t ? all[c] + sg[k][j] : sg[k][j];
+                all[cols + c] = t ? all[cols + c] + ss[k][j] : ss[k][j];
+            }
         }
     }
+    __syncthreads();
+    for (int c = threadIdx.x; c < cols; c += STREAM_THREADS) { part[c] = all[c]; part[p.n + c] = all[cols + c]; }
 }
+#undef NK_EACH
 
 // ---- rows of any length: cut into chunks of NORM_THREADS * W * 8 elements, a CTA per chunk ---------------------------------------
 constexpr int NORM_NV = 8;
@@ -827,18 +810,17 @@ __global__ void __launch_bounds__(NORM_THREADS) nk_norm_columns_kernel(T* out, c
         }
     }
 }
-// The groups' parts of the column sums: 32 columns per CTA, eight threads per column take every eighth group, in order, and are added in order.
+// The groups' parts of the column sums: 32 columns per CTA, 32 threads per column take every 32nd group, in order, and are added in order.
 template <class T>
-__global__ void __launch_bounds__(NORM_THREADS) nk_norm_columns_finish_kernel(T* dgain, int64_t dgain_s, T* dshift, int64_t dshift_s, const T* __restrict__ cols, int64_t n,
-                                                                              int64_t groups) {
-    __shared__ T sums[2][8][33];
+__global__ void __launch_bounds__(1024) nk_norm_columns_finish_kernel(T* dgain, int64_t dgain_s, T* dshift, int64_t dshift_s, const T* __restrict__ cols, int64_t n, int64_t groups) {
+    __shared__ T sums[2][32][33];
     const int lane = threadIdx.x & 31, slot = threadIdx.x >> 5;
     for (int64_t c0 = int64_t(blockIdx.x) * 32; c0 < n; c0 += int64_t(gridDim.x) * 32) {
         const int64_t c = c0 + lane;
         T sg = T(0), ss = T(0);
         if (c < n) {
-#pragma unroll 8
-            for (int64_t g = slot; g < groups; g += 8) { sg += cols[(g * 2) * n + c]; ss += cols[(g * 2 + 1) * n + c]; }
+#pragma unroll 4
+            for (int64_t g = slot; g < groups; g += 32) { sg += cols[(g * 2) * n + c]; ss += cols[(g * 2 + 1) * n + c]; }
         }
         __syncthreads();   // the sums of the columns before have been read
         sums[0][slot][lane] = sg;
@@ -847,7 +829,7 @@ __global__ void __launch_bounds__(NORM_THREADS) nk_norm_columns_finish_kernel(T*
         if (slot < 2 && c < n) {
             T v = sums[slot][0][lane];
 #pragma unroll
-            for (int k = 1; k < 8; k++) v += sums[slot][k][lane];
+            for (int k = 1; k < 32; k++) v += sums[slot][k][lane];
             if (slot == 0 && dgain) dgain[c * dgain_s] = v;
             if (slot == 1 && dshift) dshift[c * dshift_s] = v;
         }
@@ -908,25 +890,53 @@ int norm_launch(nk_ctx* ctx, const char* name, void (*kern)(A...), int64_t rows,
 // elements that a thread of the CTA kernels holds at most, and the longest row that they take (a cluster of eight)
 template <class T> constexpr int norm_e() { return 128 / int(sizeof(T)); }
 
-// Rows by bulk copies: enough of them that every team has some, rows that run along memory. Returns the warps of a team, 0: not this way.
-// (300 rows per SM and less, or up to 256 elements: the kernels above are as fast.)
+// Rows by bulk copies: at least two of them for every team, running along memory, and long: up to 256 elements on 16-byte boundaries a group of lanes
+// per row is as fast or faster (200000 x 200: forward 105 us against 100, backward 139 against 157; 200000 x 203, which has no such
+// boundaries: 127 against 102 and 237 against 152).
 template <class T> constexpr int stream_e() { return 64 / int(sizeof(T)); }
 struct StreamShape {
     int team, cluster, stages, stage_bytes, cols, grid;
     size_t smem;
 };
+// Clusters of CTAs of the kernels above that are resident at once (a GPU's SMs come in groups of unlike size that a cluster has to fit into: one that
+// waits for room would run by itself at the end). Looked up once per device and size.
+int stream_clusters(const nk_ctx* ctx, int size) {
+    static std::atomic<int> known[16][9];
+    if (size == 1) return ctx->prop.multiProcessorCount;
+    std::atomic<int>* slot = ctx->device < 16 ? &known[ctx->device][size] : nullptr;
+    int n = slot ? slot->load() : 0;
+    if (n > 0) return n;
+    auto* kern = nk_norm_grad_stream_kernel<float, 1, 16, 16>;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(unsigned(size));
+    cfg.blockDim = dim3(STREAM_THREADS);
+    cfg.dynamicSmemBytes = STREAM_SMEM;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(size);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SMEM) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = ctx->prop.multiProcessorCount / size / 2;
+    }
+    if (slot) slot->store(n);
+    return n;
+}
 template <class T>
-bool stream_shape(const nk_ctx* ctx, const NormPlan& p, int tensors, StreamShape* s) {
+bool stream_shape(const nk_ctx* ctx, const NormPlan& p, int tensors, bool vec, StreamShape* s) {
     constexpr int E = stream_e<T>();
-    if (p.n <= 256 || p.inner[1] != 1 || (tensors == 2 && p.inner[2] != 1) || p.inner[0] != 1 || !p.lo[0]) return false;
+    if (p.n <= (vec ? 256 : 128) || p.inner[1] != 1 || (tensors == 2 && p.inner[2] != 1) || p.inner[0] != 1 || !p.lo[0]) return false;
     s->team = 1;
     while (s->team < STREAM_WARPS && int64_t(s->team) * 32 * E < p.n) s->team *= 2;
     s->cluster = 1;
     while (s->cluster < 8 && int64_t(s->cluster) * s->team * 32 * E < p.n) s->cluster *= 2;
     if (int64_t(s->cluster) * s->team * 32 * E < p.n) return false;
     s->cols = s->cluster > 1 ? int(((p.n + s->cluster - 1) / s->cluster + 3) / 4 * 4) : int(p.n);   // even slices, on 16-byte boundaries of an aligned row
-    const int sms = ctx->prop.multiProcessorCount, teams = STREAM_WARPS / s->team;
-    s->grid = sms / s->cluster * s->cluster;
+    const int teams = STREAM_WARPS / s->team;
+    s->grid = stream_clusters(ctx, s->cluster) * s->cluster;
     if (p.rows < int64_t(s->grid / s->cluster) * teams * 2) return false;
     s->stage_bytes = int((size_t(s->cols) * sizeof(T) + 30) / 16 * 16);
     s->stages = int(STREAM_SMEM / (size_t(teams) * tensors * s->stage_bytes));
@@ -978,6 +988,7 @@ int forward_rows(nk_ctx* ctx, T* out, const T* src, const T* gain, const T* shif
 #define NK_LANES(G, EL) return norm_launch(ctx, "nk_norm_lanes_kernel", nk_norm_lanes_kernel<T, W, G, EL>, (p.rows + 256 / G - 1) / (256 / G), 256, 1, 32, out, src, gain, shift, stats, p, eps)
 #define NK_CTA(TH, EL, C) return norm_launch(ctx, "nk_norm_cta_kernel", nk_norm_cta_kernel<T, W, TH, EL>, p.rows, TH, C, 16, out, src, gain, shift, stats, p, eps)
     if (p.n <= 32) NK_LANES(8, 4);
+    if (p.n <= 64) NK_LANES(16, 4);
     if (p.n <= 128) NK_LANES(32, 4);
     if (p.n <= 256) NK_LANES(32, 8);
     if (p.n <= 512) NK_LANES(32, 16);
@@ -995,7 +1006,7 @@ int forward_rows(nk_ctx* ctx, T* out, const T* src, const T* gain, const T* shif
 template <class T, int W>
 int forward_w(nk_ctx* ctx, T* out, const T* src, const T* gain, const T* shift, T* stats, const NormPlan& p, T eps) {
     StreamShape shape;
-    if (stream_shape<T>(ctx, p, 1, &shape)) return forward_stream<T, W>(ctx, shape, out, src, gain, shift, stats, p, eps);
+    if (stream_shape<T>(ctx, p, 1, W > 1, &shape)) return forward_stream<T, W>(ctx, shape, out, src, gain, shift, stats, p, eps);
     if (p.n <= 4096 * norm_e<T>()) return forward_rows<T, W>(ctx, out, src, gain, shift, stats, p, eps);
     constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
     const int64_t chunks = (p.n + L - 1) / L;
@@ -1023,7 +1034,7 @@ struct NormGrad {
 };
 template <class T>
 int columns_finish(nk_ctx* ctx, const NormGrad<T>& a, const T* cols, int64_t n, int64_t groups) {
-    nk_norm_columns_finish_kernel<T><<<nk_grid_for(ctx, n, 32, 32), NORM_THREADS, 0, ctx->stream>>>(a.dgain, a.dgain_s, a.dshift, a.dshift_s, cols, n, groups);
+    nk_norm_columns_finish_kernel<T><<<nk_grid_for(ctx, n, 32, 32), 1024, 0, ctx->stream>>>(a.dgain, a.dgain_s, a.dshift, a.dshift_s, cols, n, groups);
     return nk_after_launch(ctx, "nk_norm_columns_finish_kernel");
 }
 template <class T, int W>
@@ -1061,6 +1072,7 @@ int backward_rows(nk_ctx* ctx, const NormGrad<T>& a, const NormPlan& p) {
         st = norm_launch(ctx, "nk_norm_grad_kernel", nk_norm_grad_kernel<T, W, TH, EL>, groups, TH, C, PER, a.out, a.err, a.src, a.gain, a.stats, part, p);              \
     } while (0)
     if (p.n <= 32) NK_LANES(8, 4, 4);
+    else if (p.n <= 64) NK_LANES(16, 4, 4);
     else if (p.n <= 128) NK_LANES(32, 4, 4);
     else if (p.n <= 256) NK_LANES(32, 8, 4);
     else if (p.n <= 1024) NK_CTA(128, 8, 1, 6);
@@ -1096,7 +1108,7 @@ int backward_stream(nk_ctx* ctx, const StreamShape& s, const NormGrad<T>& a, con
 template <class T, int W>
 int backward_w(nk_ctx* ctx, const NormGrad<T>& a, const NormPlan& p) {
     StreamShape shape;
-    if (stream_shape<T>(ctx, p, 2, &shape)) return backward_stream<T, W>(ctx, shape, a, p);
+    if (stream_shape<T>(ctx, p, 2, W > 1, &shape)) return backward_stream<T, W>(ctx, shape, a, p);
     if (p.n <= 2048 * norm_e<T>()) return backward_rows<T, W>(ctx, a, p);
     constexpr int64_t L = int64_t(NORM_THREADS) * W * NORM_NV;
     const int64_t chunks = (p.n + L - 1) / L, blocks_c = (p.n + NORM_THREADS * W - 1) / (NORM_THREADS * W);
