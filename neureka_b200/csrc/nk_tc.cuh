@@ -38,7 +38,7 @@ namespace {
 constexpr int TC_BM = 128, TC_BK = 16;                        // rows of A a CTA stages, k per stage
 constexpr int TC_THREADS = 576;                              // warp 0 producer, warp 1 tensor-core issue, warps 2..17 epilogue
 constexpr unsigned TC_TMEM_COLS = 512;                       // all of it: two accumulators of up to 128 x 256 F32 per CTA
-constexpr int TC_KC = 8;                                     // k blocks (of 16) per accumulation chunk
+constexpr int TC_KC = 8;                                     // k blocks (of 16) per accumulation chunk (a caller may want fewer)
 constexpr int TC_MAX_SPLITS = 16;
 
 // CG: CTAs that share a tile (1 or 2); BN: columns of the tile
@@ -230,6 +230,7 @@ struct TcParams {
     int tiles_m;
     int64_t units;                 // tiles * splits; unit u is part u % splits of tile u / splits
     int splits, kb_per;            // k blocks per part
+    int chunk;                     // k blocks per accumulation chunk
     float* parts;                  // splits > 1: [tile][part][warp of 16][columns / 4][32 rows x 4]
     int* tickets;                  // splits > 1: [tile][warp of 16]
     int* status;                   // host-mapped word, set non-zero when a bounded wait ran out
@@ -380,19 +381,19 @@ nk_conv_tc_kernel(const __grid_constant__ TcMaps<Drain::DUAL> maps, const __grid
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             // ---- tensor-core issue: per stage two k-steps of 8, three products each (small terms first); a new
-            // accumulator every TC_KC stages ----
+            // accumulator every p.chunk stages ----
             int it = 0, ch = 0;
             bool ok = true;
             for (int64_t u = unit0; u < p.units && ok; u += unit_step) {
                 int kb_begin, kb_end;
                 range(u, &kb_begin, &kb_end);
-                for (int kb0 = kb_begin; kb0 < kb_end && ok; kb0 += TC_KC, ch++) {
+                for (int kb0 = kb_begin; kb0 < kb_end && ok; kb0 += p.chunk, ch++) {
                     const int b = ch & 1;
                     ok = wait_or_abort(&acc_empty[b], ((unsigned(ch) >> 1) & 1u) ^ 1u);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t acc = tmem_base + uint32_t(b) * BN;
-                    const int kb1 = kb0 + TC_KC < kb_end ? kb0 + TC_KC : kb_end;
+                    const int kb1 = kb0 + p.chunk < kb_end ? kb0 + p.chunk : kb_end;
                     for (int kb = kb0; kb < kb1 && ok; kb++, it++) {
                         const int s = it % STAGES;
                         ok = wait_or_abort(&full_bar[s], (unsigned(it) / STAGES) & 1u);
@@ -432,7 +433,7 @@ nk_conv_tc_kernel(const __grid_constant__ TcMaps<Drain::DUAL> maps, const __grid
             const int64_t m = int64_t(t % p.tiles_m) * C::TM + rank * TC_BM + q * 32 + lane;
             const int64_t n0 = int64_t(t / p.tiles_m) * COLS + quarter * (DUAL ? EC / 2 : EC);
             float sum[EC];
-            for (int kb0 = kb_begin; kb0 < kb_end && ok; kb0 += TC_KC, ch++) {
+            for (int kb0 = kb_begin; kb0 < kb_end && ok; kb0 += p.chunk, ch++) {
                 const int b = ch & 1;
                 ok = wait_or_abort(&acc_full[b], (unsigned(ch) >> 1) & 1u);
                 if (!ok) break;
@@ -537,6 +538,7 @@ inline TcParams tc_params(const TcShape& s, int64_t M, int64_t Kp, float* parts,
     p.units = s.tiles * s.splits;
     p.splits = s.splits;
     p.kb_per = s.kb_per;
+    p.chunk = TC_KC;
     p.parts = parts;
     p.tickets = tickets;
     p.status = status;
