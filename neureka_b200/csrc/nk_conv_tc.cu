@@ -77,6 +77,7 @@ int nk_conv_tc_try(nk_ctx* ctx, nk_buf* drn, nk_buf* s1, nk_buf* s2, const GemmP
     TcPlainDrain drain;
     memset(&drain, 0, sizeof(drain));
     drain.out = static_cast<float*>(drn->ptr);
+    drain.M = p.M;
     drain.N = p.N;
     if (tables) { drain.offOm = tab + p.M; drain.offOn = tab + 2 * p.M + p.N; }
     drain.sOm = stride(p.m, true);

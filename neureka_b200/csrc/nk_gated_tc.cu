@@ -16,66 +16,108 @@ __device__ __forceinline__ void store8(float* at, const float* v) {
     asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(at), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]),
                  "f"(v[7]) : "memory");
 }
+// 16 columns of a warp's 32 rows, a lane per row, into rows of memory that no vector fits (their length is odd, or their base): stored as they are, every
+// access would touch 32 rows, so the two 16 x 16 halves are turned first, after which an access covers 16 columns of two rows. 1023 x 777 x 2051
+// forward: the product 51 -> 41 us, dW 70 -> 50 us.
+__device__ __forceinline__ void store_turned(float* base, int64_t rs, int64_t m, int64_t n0, int64_t M, int64_t N, float (&v)[16]) {
+    const int lane = threadIdx.x & 31, c = lane & 15;
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) {
+        const bool up = lane & s;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            if (j & s) continue;
+            const float got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j | s], s);
+            if (up) v[j] = got;
+            else v[j | s] = got;
+        }
+    }
+    const int64_t first = m - c;   // the row of the first lane of this half
+    float* at = base + first * rs + n0 + c;
+    if (n0 + c >= N) return;
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+        if (first + j < M) at[j * rs] = v[j];
+}
+// ... whatever the layout (called by whole warps; rows from M on are not there)
+__device__ __forceinline__ void store16(float* base, int64_t rs, int64_t cs, int vec, int64_t m, int64_t n0, int64_t M, int64_t N, float (&v)[16]) {
+    if (n0 >= N) return;
+    if (cs == 1 && !vec) store_turned(base, rs, m, n0, M, N, v);
+    else if (m >= M) return;
+    else if (vec && n0 + 16 <= N) {
+        store8(base + m * rs + n0, v);
+        store8(base + m * rs + n0 + 8, v + 8);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (n0 + i < N) base[m * rs + (n0 + i) * cs] = v[i];
+    }
+}
 // f(g) * u, and g and u where they are kept
 template <int FUN>
 struct GatedDrain {
     static constexpr bool DUAL = true;
     float *y, *gate, *up;
-    int64_t N, rs, cs;
+    int64_t M, N, rs, cs;
     int vec, kept_vec;   // 32-byte stores: the rows of y; of gate and up
     template <int EC>
-    __device__ __forceinline__ void store(int64_t m, int64_t n0, const float (&sum)[EC]) const {
+    __device__ __forceinline__ void store(int64_t m, int64_t n0, float (&sum)[EC]) const {
         constexpr int HC = EC / 2;
 #pragma unroll
-        for (int j = 0; j < HC; j += 8) {
-            const int64_t n = n0 + j;
-            if (n >= N) continue;
-            float v[8];
+        for (int j = 0; j < HC; j += 16) {
+            float v[16];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = nkf::fun(FUN, false, sum[j + i]) * sum[HC + j + i];
-            if (vec && n + 8 <= N) store8(y + m * rs + n, v);
-            else {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (n + i < N) y[m * rs + (n + i) * cs] = v[i];
-            }
-            if (!gate) continue;
-            if (kept_vec) {
-                store8(gate + m * N + n, sum + j);
-                store8(up + m * N + n, sum + HC + j);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (n + i < N) { gate[m * N + n + i] = sum[j + i]; up[m * N + n + i] = sum[HC + j + i]; }
-            }
+            for (int i = 0; i < 16; i++) v[i] = gate_fun<float>(FUN, false, sum[j + i]) * sum[HC + j + i];
+            store16(y, rs, cs, vec, m, n0 + j, M, N, v);
         }
+        if (!gate) return;
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int j = 0; j < HC; j += 16) {
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) v[i] = sum[b * HC + j + i];
+                store16(b ? up : gate, N, 1, kept_vec, m, n0 + j, M, N, v);
+            }
     }
 };
 // both products as they are; either may be unwanted
 struct TwoDrain {
     static constexpr bool DUAL = true;
     float* out[2];
-    int64_t N, rs[2], cs[2];
+    int64_t M, N, rs[2], cs[2];
     int vec[2];          // 32-byte stores along the rows
     template <int EC>
-    __device__ __forceinline__ void store(int64_t m, int64_t n0, const float (&sum)[EC]) const {
+    __device__ __forceinline__ void store(int64_t m, int64_t n0, float (&sum)[EC]) const {
         constexpr int HC = EC / 2;
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             if (!out[b]) continue;
-            float* row = out[b] + m * rs[b];
 #pragma unroll
-            for (int j = 0; j < HC; j += 8) {
-                const int64_t n = n0 + j;
-                if (n >= N) continue;
-                const float* v = sum + b * HC + j;
-                if (vec[b] && n + 8 <= N) store8(row + n, v);
-                else {
+            for (int j = 0; j < HC; j += 16) {
+                float v[16];
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (n + i < N) row[(n + i) * cs[b]] = v[i];
-                }
+                for (int i = 0; i < 16; i++) v[i] = sum[b * HC + j + i];
+                store16(out[b], rs[b], cs[b], vec[b], m, n0 + j, M, N, v);
             }
+        }
+    }
+};
+// one product
+struct OneDrain {
+    static constexpr bool DUAL = false;
+    float* out;
+    int64_t M, N, rs, cs;
+    int vec;
+    template <int EC>
+    __device__ __forceinline__ void store(int64_t m, int64_t n0, float (&sum)[EC]) const {
+#pragma unroll
+        for (int j = 0; j < EC; j += 16) {
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = sum[j + i];
+            store16(out, rs, cs, vec, m, n0 + j, M, N, v);
         }
     }
 };
@@ -121,8 +163,8 @@ __global__ void __launch_bounds__(256) nk_gated_errors_split_kernel(const GatedC
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            d[0][j] = e[j] * u[j] * nkf::fun(FUN, true, g[j]);
-            d[1][j] = e[j] * nkf::fun(FUN, false, g[j]);
+            d[0][j] = e[j] * u[j] * gate_fun<float>(FUN, true, g[j]);
+            d[1][j] = e[j] * gate_fun<float>(FUN, false, g[j]);
 #pragma unroll
             for (int b = 0; b < 2; b++) tile[b][warp + 8 * i][lane * 4 + j] = d[b][j];
         }
@@ -185,8 +227,9 @@ int split(nk_ctx* ctx, const TcSplit& sp) {
     return nk_after_launch(ctx, "nk_tc_split_kernel");
 }
 // Chunks of 128 k leave a result 1.8e-6 off (2-norm, normal operands; the accumulator truncates), chunks of 64 k 0.9e-6, whatever the length of the
-// sum; a sum of F32 multiply-adds is 2.7e-8 sqrt(K) off. So sums of up to 4096 take the shorter chunks, which cost a fifth of the time (accumulators
-// are read out twice as often: 4096 x 2048 x 8192 forward 1.23 -> 1.50 ms), and longer ones lose nothing by the longer ones.
+// sum; a sum of F32 multiply-adds is 2.7e-8 sqrt(K) off. So sums of up to 4096 take the shorter chunks, which cost a tenth of the time (accumulators
+// are read out twice as often, and a tile's stores hide behind half as much: 4096 x 2048 x 8192 forward 1.18 -> 1.30 ms), and longer ones lose
+// nothing by the longer ones.
 template <class Drain>
 int product(nk_ctx* ctx, const TcShape& shape, int64_t Kp, const TcPanels& a, const TcPanels& b0, const TcPanels& b1, TcParams tp, const Drain& drain) {
     if (Kp < 4096) tp.chunk = TC_KC / 2;
@@ -230,7 +273,7 @@ int nk_gated_tc_forward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     const TcParams tp = tc_params(shape, c.T, Kp, at(parts), sp.tickets, ctx->tma_status_dev);
     const TcPanels a{at(x_hi), at(x_lo), c.T}, b0{at(g_hi), at(g_lo), c.H}, b1{at(u_hi), at(u_lo), c.H};
     const int kept_vec = c.H % 8 == 0 && reinterpret_cast<uintptr_t>(c.gate) % 32 == 0 && reinterpret_cast<uintptr_t>(c.up) % 32 == 0;
-#define NK_CASE(FUN) st = product(ctx, shape, Kp, a, b0, b1, tp, GatedDrain<FUN>{static_cast<float*>(c.y.ptr), static_cast<float*>(c.gate), static_cast<float*>(c.up), c.H, c.y.rs, c.y.cs, wide_rows(c.y), kept_vec})
+#define NK_CASE(FUN) st = product(ctx, shape, Kp, a, b0, b1, tp, GatedDrain<FUN>{static_cast<float*>(c.y.ptr), static_cast<float*>(c.gate), static_cast<float*>(c.up), c.T, c.H, c.y.rs, c.y.cs, wide_rows(c.y), kept_vec})
     NK_GATE_SWITCH(c.fun, NK_CASE)
 #undef NK_CASE
     *handled = true;
@@ -301,19 +344,14 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     if (dx && narrow) {
         if ((st = nk_gated_narrow_dx_panels(ctx, c, at(a_hi), at(a_lo), at(px), ep.tickets))) return st;
     } else if (dx) {
-        TcPlainDrain drain;
-        memset(&drain, 0, sizeof(drain));
-        drain.out = static_cast<float*>(c.dx.ptr);
-        drain.N = c.D;
-        drain.sOm = c.dx.rs;
-        drain.sOn = c.dx.cs;
-        drain.out_vec = vec_rows(c.dx);
+        const OneDrain drain{static_cast<float*>(c.dx.ptr), c.T, c.D, c.dx.rs, c.dx.cs, wide_rows(c.dx)};
         const TcPanels a{at(a_hi), at(a_lo), c.T}, b{at(w_hi), at(w_lo), c.D};
         if ((st = product(ctx, sx, 2 * Hp, a, b, b, tc_params(sx, c.T, 2 * Hp, at(px), ep.tickets, ctx->tma_status_dev), drain))) return st;
     }
     if (dw) {
         TwoDrain drain;
         memset(&drain, 0, sizeof(drain));
+        drain.M = c.D;
         drain.N = c.H;
         for (int b = 0; b < 2; b++) {
             drain.out[b] = static_cast<float*>(c.dw[b].ptr);

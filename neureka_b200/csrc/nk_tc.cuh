@@ -241,18 +241,20 @@ struct TcMaps {
     CUtensorMap a[2], b[DUAL ? 4 : 2];
 };
 
-// What becomes of a tile's sums. A drain with DUAL = false takes a thread's row m and 32-column groups of its EC columns from n0 on. With
+// What becomes of a tile's sums. A drain is called by whole warps (rows past
+// the last among them). One with DUAL = false takes a thread's row m and 32-column groups of its EC columns from n0 on. With
 // DUAL = true there are two B operands of one shape, a tile is BN / 2 columns of each product, and a thread holds its row's columns [n0, n0 + EC / 2)
 // of the first product and then of the second.
 struct TcPlainDrain {
     static constexpr bool DUAL = false;
     float* out;
-    int64_t N;
+    int64_t M, N;
     const int64_t *offOm, *offOn;  // null: m * sOm, n * sOn
     int64_t sOm, sOn, bO;
     int out_vec;                   // the drain's n index is its contiguous direction and every row starts 16-byte aligned
     template <int EC>
     __device__ __forceinline__ void store(int64_t m, int64_t n0, const float (&sum)[EC]) const {
+        if (m >= M) return;
         const int64_t row = bO + (offOm ? offOm[m] : m * sOm);
 #pragma unroll
         for (int c = 0; c < EC / 32; c++) {
@@ -483,7 +485,7 @@ nk_conv_tc_kernel(const __grid_constant__ TcMaps<Drain::DUAL> maps, const __grid
                     }
                 }
             }
-            if (m < p.M) drain.store(m, n0, sum);
+            drain.store(m, n0, sum);
         }
     }
 
