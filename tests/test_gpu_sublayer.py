@@ -449,3 +449,231 @@ def test_refusals(device):
     assert ggrad() == L.NK_OK and ggrad(d=N) == L.NK_OK
     assert ggrad(k=None) == BAD and ggrad(k=stats._data.buf) == OUT and ggrad(e=b(x)) == BAD and ggrad(g=b(x)) == BAD and ggrad(d=virtual) == BAD
     device.sync()
+
+
+# ---- calls that are seldom made ----------------------------------------------------------------------------------------------------
+class Raw:
+    """Buffers of torch's memory for the C entry points"""
+
+    def __init__(self, ctx):
+        self.ctx, self.keep = ctx, []
+
+    def __call__(self, values, shape=None, strides=None):
+        """a buffer with these values, and the view of it (dense, or of the given shape and strides)"""
+        import torch
+        t = torch.as_tensor(values, device="cuda").contiguous()
+        buf = C.c_void_p()
+        L.check(L.lib.nk_wrap(self.ctx, L.NK_F32 if t.dtype == torch.float32 else L.NK_F64, C.c_void_p(t.data_ptr()), t.numel(), C.byref(buf)), self.ctx)
+        shape = list(t.shape) if shape is None else list(shape)
+        dense = [int(np.prod(shape[k + 1:])) for k in range(len(shape))]
+        arr = np.array(shape + (dense if strides is None else list(strides)) + dense + [0] * len(shape) + [1] * len(shape), dtype=np.int32)
+        self.keep.append((t, arr))
+        return t, (buf, arr.ctypes.data_as(C.POINTER(C.c_int32)))
+
+
+def sub_layer_calls(ctx, dtype, t, d, h):
+    """One pass through everything, forward and backward, on ctx's stream: the inputs, the results, and the calls as a function"""
+    import torch
+    raw, dt = Raw(ctx), L.NK_F32 if dtype == np.float32 else L.NK_F64
+    rng = np.random.default_rng(t + d + h)
+    (x, bx), (e, be) = (raw(rng.standard_normal((t, d)).astype(dtype)) for _ in range(2))
+    (wg, bwg), (wu, bwu) = (raw((rng.standard_normal((d, h)) / np.sqrt(d)).astype(dtype)) for _ in range(2))
+    (wd, bwd), (gain, bgain) = raw(rng.standard_normal((t, h)).astype(dtype)), raw(1 + 0.1 * rng.standard_normal(d).astype(dtype))
+    (n, bn), (stats, bstats), (y, by), (kept, bkept), (o, bo) = (raw(np.zeros(s, dtype)) for s in ((t, d), (2, t), (t, h), (2, t, h), (t, h)))
+    (dn, bdn), (dg, bdg), (du, bdu), (dx, bdx), (dgain, bdgain), (dshift, bdshift) = (raw(np.zeros(s, dtype)) for s in ((t, d), (d, h), (d, h), (t, d), (d,), (d,)))
+    N, lib, silu = (None, None), L.lib, L.FUN["silu"]
+
+    def run():
+        L.check(lib.nk_layer_norm(ctx, dt, 2, *bn, *bx, *bgain, *N, 1e-5, bstats[0]), ctx)
+        L.check(lib.nk_gated(ctx, silu, dt, *by, *bn, *bwg, *bwu, bkept[0]), ctx)
+        L.check(lib.nk_dropout(ctx, dt, 2, *bo, *by, *bwd, 0.25, 7, 8), ctx)
+        L.check(lib.nk_gated_grad(ctx, silu, dt, *bdn, *bdg, *bdu, *bo, *bn, *bwg, *bwu, bkept[0]), ctx)
+        L.check(lib.nk_layer_norm_grad(ctx, dt, 2, *bdx, *bdgain, *bdshift, *bdn, *bx, *bgain, bstats[0]), ctx)
+    torch.cuda.synchronize()
+    return (x, wg), (n, y, o, dg, du, dx, dgain, dshift), run, raw
+
+
+SUB_LAYERS = [(np.float32, 1, 128, 200), (np.float32, 24, 300, 257), (np.float32, 300, 260, 515), (np.float32, 3000, 640, 100), (np.float64, 5, 70, 96), (np.float64, 200, 130, 70),
+              (np.float32, 2, 140000, 20)]
+
+
+@pytest.mark.parametrize("case", SUB_LAYERS, ids=lambda c: f"{c[0].__name__}-{c[1]}-{c[2]}-{c[3]}")
+def test_captured_once_and_replayed(device, case):
+    import torch
+    (x, wg), results, run, raw = sub_layer_calls(device.ctx, *case)
+    stream = torch.cuda.ExternalStream(L.lib.nk_stream(device.ctx))
+    run()   # (what is looked up once per device has been)
+    device.sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+        run()
+    for k in range(3):   # other values in the same places
+        x.mul_(0.75).add_(0.125)
+        wg.mul_(-1.25)
+        torch.cuda.synchronize()
+        run()
+        device.sync()
+        want = [r.clone() for r in results]
+        for r in results:
+            r.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+            if k == 2:
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(results, want))
+
+
+def test_two_graphs_and_eager_calls_at_work_at_once(device):
+    import torch
+    second = C.c_void_p()
+    L.check(L.lib.nk_device_open(device.ordinal, C.byref(second)))
+    try:
+        sides = []
+        for ctx, case in ((device.ctx, (np.float32, 300, 260, 515)), (second, (np.float32, 24, 300, 257)), (second, (np.float32, 500, 200, 300))):
+            _, results, run, raw = sub_layer_calls(ctx, *case)
+            run()
+            L.check(L.lib.nk_sync(ctx), ctx)
+            want, stream = [r.clone() for r in results], torch.cuda.ExternalStream(L.lib.nk_stream(ctx))
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+                run()
+            sides.append((results, want, graph, torch.cuda.Stream(), run, raw))
+        for k in range(10):
+            for results, want, graph, own, run, raw in sides:
+                with torch.cuda.stream(own):   # a stream of its own: the graphs have memory of their own
+                    graph.replay()
+            torch.cuda.synchronize()
+            for results, want, graph, own, run, raw in sides:
+                assert all(torch.equal(a, b) for a, b in zip(results, want))
+        for k in range(10):   # both contexts, eagerly
+            for results, want, graph, own, run, raw in sides:
+                run()
+        torch.cuda.synchronize()
+        for results, want, graph, own, run, raw in sides:
+            assert all(torch.equal(a, b) for a, b in zip(results, want))
+        del sides, results, want, graph, own, run, raw
+    finally:
+        L.lib.nk_device_close(second)
+
+
+@pytest.mark.parametrize("size", [(1, 70, 90), (5, 64, 48), (24, 96, 130), (200, 260, 300)], ids=str)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gated_of_one_value_standing_for_many(device, dtype, size):
+    """rows or whole matrices that are one row or one value in memory, as operands and as the error"""
+    t, d, h = size
+    rng, raw, dt, ctx = np.random.default_rng(41), Raw(device.ctx), L.NK_F32 if dtype == np.float32 else L.NK_F64, device.ctx
+    vx, vg, vu, ve = rng.standard_normal(d).astype(dtype), (rng.standard_normal(h) / d).astype(dtype), np.array([0.5 / d], dtype), np.array([0.75], dtype)
+    x, wg, wu, e = np.tile(vx, (t, 1)), np.tile(vg, (d, 1)), np.full((d, h), vu[0]), np.full((t, h), ve[0])
+    _, bx = raw(vx, (t, d), (0, 1))
+    _, bg = raw(vg, (d, h), (0, 1))
+    _, bu = raw(vu, (d, h), (0, 0))
+    _, be = raw(ve, (t, h), (0, 0))
+    (y, by), (kept, bk), (dx, bdx), (dg, bdg), (du, bdu) = (raw(np.zeros(s, dtype)) for s in ((t, h), (2, t, h), (t, d), (d, h), (d, h)))
+    import torch
+    torch.cuda.synchronize()
+    L.check(L.lib.nk_gated(ctx, L.FUN["gelu"], dt, *by, *bx, *bg, *bu, bk[0]), ctx)
+    L.check(L.lib.nk_gated_grad(ctx, L.FUN["gelu"], dt, *bdx, *bdg, *bdu, *be, *bx, *bg, *bu, bk[0]), ctx)
+    device.sync()
+    S.assert_within(y.cpu().numpy(), S.gated(x, wg, wu, "gelu")[0], "y")
+    for name, got, want in zip(("dx", "dwg", "dwu"), (dx, dg, du), S.gated_gradients(x, wg, wu, e, "gelu")):
+        S.assert_within(got.cpu().numpy(), want, name)
+
+
+def test_one_leaf_in_every_place(device):
+    """The same tensor as several operands: its gradients add up."""
+    rng = np.random.default_rng(42)
+    u = S.unit(np.float64)
+    a, e = rng.standard_normal((60, 60)) / 4, rng.standard_normal((60, 60))
+    ta = put(device, a).set_rqs_gradient(True)
+    ta.gated(ta, ta, "tanh").backward(put(device, e))
+    parts = S.gated_gradients(a, a, a, e, "tanh")
+    want, bound = sum(p[0] for p in parts), sum(p[1] for p in parts)
+    S.assert_within(ta.gradient.numpy(), (want, bound + 3 * u * sum(np.abs(p[0]) for p in parts)), "a")
+    x, v, e = rng.standard_normal((30, 40)), rng.standard_normal(40), rng.standard_normal((30, 40))
+    tx, tv = put(device, x), put(device, v).set_rqs_gradient(True)
+    tx.layer_norm(tv, tv).backward(put(device, e))
+    _, dgain, dshift = S.norm_gradients(x, v, e, 1e-5, u)
+    S.assert_within(tv.gradient.numpy(), (dgain[0] + dshift[0], dgain[1] + dshift[1] + 2 * u * (np.abs(dgain[0]) + np.abs(dshift[0]))), "v")
+    tx = put(device, x).set_rqs_gradient(True)
+    y = tx.dropout(0.5, 3, 4, residual=tx)
+    assert np.array_equal(y.numpy(), S.dropout(x, 0.5, 3, 4, x))
+    y.backward(put(device, e))
+    assert np.array_equal(tx.gradient.numpy(), e + S.dropout(e, 0.5, 3, 4))
+
+
+def test_backward_without_an_error(device):
+    """ones, one value standing for all"""
+    rng = np.random.default_rng(43)
+    x, wg, wu = rng.standard_normal((20, 30)), rng.standard_normal((30, 50)) / 5, rng.standard_normal((30, 50)) / 5
+    tx, tg, tu = (put(device, a).set_rqs_gradient(True) for a in (x, wg, wu))
+    tx.gated(tg, tu).backward()
+    for got, want in zip((tx, tg, tu), S.gated_gradients(x, wg, wu, np.ones((20, 50)), "silu")):
+        S.assert_within(got.gradient.numpy(), want, "gated")
+    gain = 1 + rng.standard_normal(30)
+    tx, tg = put(device, x).set_rqs_gradient(True), put(device, gain).set_rqs_gradient(True)
+    tx.layer_norm(tg).backward()
+    dx, dgain, _ = S.norm_gradients(x, gain, np.ones((20, 30)), 1e-5, S.unit(np.float64))
+    S.assert_within(tx.gradient.numpy(), dx, "dx")
+    S.assert_within(tg.gradient.numpy(), dgain, "dgain")
+    tx = put(device, x).set_rqs_gradient(True)
+    tx.dropout(0.3, 1).backward()
+    assert np.array_equal(tx.gradient.numpy(), S.dropout(np.ones((20, 30)), 0.3, 1, 0))
+
+
+@pytest.mark.parametrize("shape", [(5000, 96), (3000, 777), (700, 4096), (320, 12001), (2, 140001)], ids=str)
+def test_layer_norm_in_place_of_many_and_of_long_rows(device, shape):
+    import torch
+    rng, raw, ctx = np.random.default_rng(44), Raw(device.ctx), device.ctx
+    x, e = rng.standard_normal(shape).astype(np.float32), rng.standard_normal(shape).astype(np.float32)
+    (tx, bx), (ty, by), (te, be), (tr, br) = (raw(a) for a in (x, x, e, e))
+    (s0, bs), (dx, bdx), (d0, bd0), (d1, bd1) = (raw(np.zeros(s, np.float32)) for s in ((2, shape[0]), shape, shape[1:], shape[1:]))
+    N = (None, None)
+    torch.cuda.synchronize()
+    for drain in (by, by):   # (the second time on what the first one left, as one after the other would)
+        L.check(L.lib.nk_layer_norm(ctx, L.NK_F32, 2, *bdx, *by, *N, *N, 1e-5, None), ctx)
+        L.check(L.lib.nk_layer_norm(ctx, L.NK_F32, 2, *drain, *by, *N, *N, 1e-5, None), ctx)
+    device.sync()
+    assert torch.equal(ty, dx)
+    L.check(L.lib.nk_layer_norm(ctx, L.NK_F32, 2, *bdx, *bx, *N, *N, 1e-5, bs[0]), ctx)
+    L.check(L.lib.nk_layer_norm_grad(ctx, L.NK_F32, 2, *bdx, *bd0, *N, *be, *bx, *N, bs[0]), ctx)
+    L.check(L.lib.nk_layer_norm_grad(ctx, L.NK_F32, 2, *br, *bd1, *N, *br, *bx, *N, bs[0]), ctx)
+    device.sync()
+    assert torch.equal(tr, dx) and torch.equal(d0, d1)
+    S.assert_within(tr.cpu().numpy(), S.norm_gradients(x, None, e, 1e-5, S.unit(np.float32))[0], "dx")
+
+
+@pytest.mark.parametrize("fun", L.GATES)
+def test_f32_gates_over_their_whole_range(device, fun):
+    """x = [v, 1] with weights [1, 0] and [0, 1] (in one tile of F32 multiply-adds: exact) give g = v, u = 1, y = f(v) and, for an error of ones,
+    dx = [f'(v), f(v)]. With e = e^-|k v|: 4 u for e (2 units in the last place), 4 for the quotient, 1 each for 1 + e, e t, v s, 2 for e's share in 1 + e,
+    and 3 for gelu's correction: 16 u; the derivatives have two such factors and three operations more: 36 u of their terms."""
+    v = np.concatenate([np.linspace(-20, 20, 4001), np.linspace(-120, 120, 999), np.geomspace(1e-30, 3e38, 400), -np.geomspace(1e-30, 3e38, 400), [0.0, -0.0]]).astype(np.float32)
+    x = np.stack([v, np.ones_like(v)], 1)
+    tx = put(device, x).set_rqs_gradient(True)
+    y = tx.gated(put(device, np.array([[1], [0]], np.float32)), put(device, np.array([[0], [1]], np.float32)), fun)
+    y.backward()
+    w, u = v.astype(S.WIDE), S.unit(np.float32)
+    if fun in ("idy", "relu"):
+        f, df = S.gate(fun, v)
+        f_off, df_off = 2 * u * np.abs(f), 2 * u * np.abs(df)
+    else:
+        k = S.WIDE({"gelu": 1.702, "tanh": 2}.get(fun, 1))
+        e = np.exp(-k * np.abs(w))
+        small, large = e / (1 + e), 1 / (1 + e)
+        s, rest = np.where(w < 0, small, large), np.where(w < 0, large, small)
+        if fun == "tanh":
+            f, df = np.tanh(w), 4 * s * rest
+            terms = df
+        elif fun == "sig":
+            f, df = s, s * rest
+            terms = df
+        else:
+            f, df = w * s, s + k * w * s * rest
+            terms = s + k * np.abs(w) * s * rest
+        f_off, df_off = 16 * u * np.abs(f), 36 * u * terms
+    denormal = 2.0 ** -146   # what a result, or a factor of it, may be off by where it is below the normal range
+    S.assert_within(y.numpy()[:, 0], (f, f_off + denormal * (1 + np.minimum(np.abs(w), 200))), "f")
+    S.assert_within(tx.gradient.numpy()[:, 1], (f, f_off + denormal * (1 + np.minimum(np.abs(w), 200))), "f again")
+    S.assert_within(tx.gradient.numpy()[:, 0], (df, df_off + denormal * (1 + 2 * np.minimum(np.abs(w), 200))), "f'")
