@@ -46,7 +46,7 @@ __device__ __forceinline__ float gate_fun32(int f, bool derive, float x) {
         rest = fmaf(-at * rest, left, rest);
     }
     if (f == NK_FUN_SIG) return derive ? s * rest : s;
-    return derive ? fmaf(a * s, rest, s) : x * s;
+    return derive ? fmaf(fminf(fmaxf(a, -128.0f), 128.0f) * rest, s, s) : x * s;   // (rest or s is 0 beyond, and 1.702 x may be infinite)
 }
 template <class T>
 __device__ __forceinline__ T gate_fun(int f, bool derive, T x) {
