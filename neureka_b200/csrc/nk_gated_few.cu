@@ -64,7 +64,9 @@ __global__ void __launch_bounds__(FEW_THREADS) nk_gated_few_kernel(const FewCall
         }
         __syncthreads();
         if constexpr (!TURNED) {
-            constexpr int U = 4;
+            // F32 vectors of one token: 16 loads in flight (4096 x 8192: 47 us, with 8 60); without vectors they are 64 and cost registers (2048 x 5461: 34 us
+            // against 25), F64 gains nothing
+            constexpr int U = TOK == 1 && VEC && sizeof(T) == 4 ? 8 : 4;
             for (int k = warp * U; k < kc; k += FEW_WARPS * U) {
                 T wv[U][2][V];
 #pragma unroll
