@@ -10,6 +10,7 @@
 #include <cooperative_groups.h>
 
 #include "nk_gated.cuh"
+#include "nk_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -101,14 +102,19 @@ __global__ void __launch_bounds__(256) nk_gated_tile_kernel(const GatedTile p) {
 // mma.m8n8k4, 64 x 64 tiles of four warps with 32 x 32 each (nk_conv_gemm.cu: why). With two B operands the tile is 32 columns of each product and
 // the blocks of eight columns alternate between the two, so that a thread holds both products of an element. k is split over the CTAs of a
 // cluster where the tiles are few; the tile passes through shared memory at the end, where the cluster's parts meet in rank order.
+// Panels are copied asynchronously, element by element (any strides), two ahead (held in registers between load and store, one ahead: 1000 x 1000 x
+// 1000 forward 230 us, now 217). That is 18.4 TFLOP/s; 32 multiply-adds a clock and multiprocessor, which the matrix instructions seem to end at
+// (16 x 8 x 8 ones give the same), would be 18.6. 300 x 512 x 1365 forward: 44 us.
 constexpr int GD_T = 64, GD_K = 16, GD_PITCH = 20;   // a panel's rows have a pitch of 20 doubles: the fragment loads of a half warp fall on 16 banks
+constexpr int GD_RING = 3, GD_SMEM = GD_RING * 2 * GD_T * GD_PITCH * int(sizeof(double));
 __device__ __forceinline__ void gd_mma(double (&c)[2], double a, double b) {
     asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
 }
 template <int MODE>
 __global__ void __launch_bounds__(128, 3) nk_gated_dmma_kernel(const GatedTile p) {
     constexpr int COLS = MODE == GATED_SUM ? GD_T : GD_T / 2;   // columns of an output that a tile covers
-    __shared__ double smem[2 * 2 * GD_T * GD_PITCH];            // [buffer][A, B][row][k]; then the tile, [row][column]
+    extern __shared__ __align__(16) unsigned char gd_smem[];    // [buffer][A, B][row][k]; then the tile, [row][column]
+    double* smem = reinterpret_cast<double*>(gd_smem);
     auto As = reinterpret_cast<double (*)[2][GD_T][GD_PITCH]>(smem);
     cg::cluster_group cluster = cg::this_cluster();
     const int size = int(cluster.num_blocks()), rank = int(cluster.block_rank());
@@ -118,7 +124,6 @@ __global__ void __launch_bounds__(128, 3) nk_gated_dmma_kernel(const GatedTile p
     // panels of 16 k, of both phases of a SUM one after the other; this CTA's share of them
     const int64_t phase_panels = (p.K + GD_K - 1) / GD_K, panels = phase_panels * (MODE == GATED_SUM ? 2 : 1);
     const int64_t first = rank * panels / size, last = (rank + 1) * panels / size;
-    double ra[8], rb[8];
     // Element i of a thread's share of a panel, the operand's contiguous direction across the threads: k = tid % 16 and rows tid / 16 + 8 i where k is,
     // otherwise row tid % 64 and k = tid / 64 + 2 i. An element's address is one base per thread plus a constant step, moved on by a
     // panel at a time (worked out per element, the integer chains took longer than the products).
@@ -157,30 +162,34 @@ __global__ void __launch_bounds__(128, 3) nk_gated_dmma_kernel(const GatedTile p
             wb[0] = walk(B, B.cs, B.rs, false, n0 + (r >> 4) * 8 + (r & 7) - r, p.N, 8, 8, k0);
         }
     };
-    auto fetch = [&](int64_t panel) {
+    const double *any_a = static_cast<const double*>(p.a[0].ptr), *any_b = static_cast<const double*>(p.b[0].ptr);   // (not read where there is no element: zeros)
+    auto fetch = [&](int64_t panel, int buf) {
         const int phase = MODE == GATED_SUM && panel >= phase_panels;
         const int64_t k0 = (panel - phase * phase_panels) * GD_K;
         if (panel == first || (MODE == GATED_SUM && panel == phase_panels)) start(phase, k0);
         const int left = p.K - k0 < GD_K ? int(p.K - k0) : GD_K, ak = a_kfast ? tid & 15 : tid >> 6, bk = b_kfast ? tid & 15 : tid >> 6;
 #pragma unroll
-        for (int i = 0; i < 8; i++) ra[i] = ((wa.rows >> i) & 1u) && ak + (a_kfast ? 0 : 2 * i) < left ? wa.at[i * wa.step] : 0.0;
+        for (int i = 0; i < 8; i++) {
+            const bool in = ((wa.rows >> i) & 1u) && ak + (a_kfast ? 0 : 2 * i) < left;
+            nk_cp_async_8(&As[buf][0][a_kfast ? (tid >> 4) + 8 * i : tid & 63][a_kfast ? tid & 15 : (tid >> 6) + 2 * i], in ? wa.at + i * wa.step : any_a, in ? 8 : 0);
+        }
         wa.at += wa.panel;
         if (MODE != GATED_SUM && b_kfast) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) rb[i] = ((wb[i & 1].rows >> (i >> 1)) & 1u) && bk < left ? wb[i & 1].at[(i >> 1) * wb[i & 1].step] : 0.0;
+            for (int i = 0; i < 8; i++) {
+                const Walk& w = wb[i & 1];
+                const bool in = ((w.rows >> (i >> 1)) & 1u) && bk < left;
+                nk_cp_async_8(&As[buf][1][(tid >> 4) + 8 * i][tid & 15], in ? w.at + (i >> 1) * w.step : any_b, in ? 8 : 0);
+            }
             wb[1].at += wb[1].panel;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) rb[i] = ((wb[0].rows >> i) & 1u) && bk + (b_kfast ? 0 : 2 * i) < left ? wb[0].at[i * wb[0].step] : 0.0;
+            for (int i = 0; i < 8; i++) {
+                const bool in = ((wb[0].rows >> i) & 1u) && bk + (b_kfast ? 0 : 2 * i) < left;
+                nk_cp_async_8(&As[buf][1][b_kfast ? (tid >> 4) + 8 * i : tid & 63][b_kfast ? tid & 15 : (tid >> 6) + 2 * i], in ? wb[0].at + i * wb[0].step : any_b, in ? 8 : 0);
+            }
         }
         wb[0].at += wb[0].panel;
-    };
-    auto stash = [&](int buf) {   // (what the last fetch brought, by the same places)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            As[buf][0][a_kfast ? (tid >> 4) + 8 * i : tid & 63][a_kfast ? tid & 15 : (tid >> 6) + 2 * i] = ra[i];
-            As[buf][1][b_kfast ? (tid >> 4) + 8 * i : tid & 63][b_kfast ? tid & 15 : (tid >> 6) + 2 * i] = rb[i];
-        }
     };
     double acc[4][4][2];
 #pragma unroll
@@ -188,15 +197,17 @@ __global__ void __launch_bounds__(128, 3) nk_gated_dmma_kernel(const GatedTile p
 #pragma unroll
         for (int j = 0; j < 4; j++) acc[i][j][0] = acc[i][j][1] = 0.0;
     const int wm = (warp >> 1) * 32, wn = (warp & 1) * 32, fr = lane >> 2, fk = lane & 3;
-    if (first < last) {
-        fetch(first);
-        stash(0);
+#pragma unroll
+    for (int q = 0; q < GD_RING - 1; q++) {
+        if (first + q < last) fetch(first + q, q);
+        nk_cp_async_commit();
     }
-    __syncthreads();
     int buf = 0;
     for (int64_t panel = first; panel < last; panel++) {
-        const bool more = panel + 1 < last;
-        if (more) fetch(panel + 1);
+        nk_cp_async_wait<GD_RING - 2>();
+        __syncthreads();   // the panel has landed for everyone, and everyone has read the one whose buffer is filled next
+        if (panel + GD_RING - 1 < last) fetch(panel + GD_RING - 1, (buf + GD_RING - 1) % GD_RING);
+        nk_cp_async_commit();
 #pragma unroll
         for (int k = 0; k < GD_K; k += 4) {
             double a[4], b[4];
@@ -209,12 +220,9 @@ __global__ void __launch_bounds__(128, 3) nk_gated_dmma_kernel(const GatedTile p
 #pragma unroll
                 for (int j = 0; j < 4; j++) gd_mma(acc[i][j], a[i], b[j]);
         }
-        if (more) {
-            stash(buf ^ 1);   // the other buffer was last read one panel ago, before the barrier below
-            __syncthreads();
-            buf ^= 1;
-        }
+        buf = buf + 1 == GD_RING ? 0 : buf + 1;
     }
+    nk_cp_async_wait<0>();
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -254,10 +262,12 @@ int launch_dmma(nk_ctx* ctx, const GatedTile& p) {
     int split = 1;
     while (split < 8 && tiles * split < int64_t(ctx->prop.multiProcessorCount) * 2 && panels / (split * 2) >= 4) split *= 2;
     if (tiles * split > 0x7fffffffLL) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_gated: a result of %lld x %lld elements is too large", (long long)p.M, (long long)p.N);
+    NK_CUDA(ctx, cudaFuncSetAttribute(nk_gated_dmma_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, GD_SMEM));
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(unsigned(tiles * split));
     cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = GD_SMEM;
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
