@@ -3,7 +3,8 @@
 //
 // Which kernels take a call:
 //   F32  1 token, or a matrix with a side below 16 and at most 8 tokens: nk_gated_few.cu; 2 to 192 tokens: nk_gated_narrow.cu; more, of at least 64 x 64
-//        weights and 2^20 multiply-adds: nk_gated_tc.cu; the rest: nk_gated_tile_kernel;
+//        weights and 2^20 multiply-adds: nk_gated_tc.cu; the rest: nk_gated_tile_kernel. dW is a sum over the tokens: at most 8 nk_gated_few.cu, up to 64
+//        and 2^26 multiply-adds nk_gated_tile_kernel, else nk_gated_tc.cu;
 //   F64  at most 8 tokens: nk_gated_few.cu; more: nk_gated_dmma_kernel.
 // Both kernels below take any sizes and any strides; both products of a tile share the panel of x and end in the same thread, so the
 // activation and the product with it need no further pass.
@@ -17,6 +18,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 // ---- the tile kernel -------------------------------------------------------------------------------------------------------------
+// For what is too small to fill the chip: bound by latency (200 x 128 x 256 forward would be 20 us, on the tensor cores 16).
 // FORWARD: C_i = A_0 B_i, out_0 = f(C_0) * C_1 (C_i kept where wanted).  TWO: out_i = A_0 B_i.  SUM: out_0 = A_0 B_0 + A_1 B_1.
 enum { GATED_FORWARD, GATED_TWO, GATED_SUM };
 struct GatedTile {
@@ -103,8 +105,8 @@ __global__ void __launch_bounds__(256) nk_gated_tile_kernel(const GatedTile p) {
 // the blocks of eight columns alternate between the two, so that a thread holds both products of an element. k is split over the CTAs of a
 // cluster where the tiles are few; the tile passes through shared memory at the end, where the cluster's parts meet in rank order.
 // Panels are copied asynchronously, element by element (any strides), two ahead (held in registers between load and store, one ahead: 1000 x 1000 x
-// 1000 forward 230 us, now 217). That is 18.4 TFLOP/s; 32 multiply-adds a clock and multiprocessor, which the matrix instructions seem to end at
-// (16 x 8 x 8 ones give the same), would be 18.6. 300 x 512 x 1365 forward: 44 us.
+// 1000 forward 230 us against 217). Bound by the FP64 matrix instructions: 2000 x 1000 x 1000 forward 316 us (25 TFLOP/s; products of 2048^3
+// reach 27), 300 x 512 x 1365 44 us, where the last wave and the first panels weigh more. 16 x 8 x 8 instructions take as long as 8 x 8 x 4 ones.
 constexpr int GD_T = 64, GD_K = 16, GD_PITCH = 20;   // a panel's rows have a pitch of 20 doubles: the fragment loads of a half warp fall on 16 banks
 constexpr int GD_RING = 3, GD_SMEM = GD_RING * 2 * GD_T * GD_PITCH * int(sizeof(double));
 __device__ __forceinline__ void gd_mma(double (&c)[2], double a, double b) {
@@ -258,9 +260,15 @@ template <int MODE>
 int launch_dmma(nk_ctx* ctx, const GatedTile& p) {
     constexpr int COLS = MODE == GATED_SUM ? GD_T : GD_T / 2;
     const int64_t tiles = ((p.M + GD_T - 1) / GD_T) * ((p.N + COLS - 1) / COLS), panels = (p.K + GD_K - 1) / GD_K * (MODE == GATED_SUM ? 2 : 1);
-    // three CTAs fit an SM: k is split, in parts of at least 64, until there are about two per SM
+    // k is split, in parts of at least 64, where that evens out the SMs' shares. Three CTAs fit an SM and share its FP64 units, one by itself leaves half of
+    // them idle, and a part costs about two panels of its own. 1000 x 1000 x 1000 forward, 512 tiles: whole 217 us, in four parts 185.
+    const int64_t sms = ctx->prop.multiProcessorCount;
     int split = 1;
-    while (split < 8 && tiles * split < int64_t(ctx->prop.multiProcessorCount) * 2 && panels / (split * 2) >= 4) split *= 2;
+    int64_t best = 0;
+    for (int s = 1; s <= 8 && (s == 1 || panels / s >= 4) && tiles < (int64_t(1) << 28); s *= 2) {
+        const int64_t per_sm = (tiles * s + sms - 1) / sms, cost = (per_sm + (per_sm % 3 == 1)) * (panels / s + 2);
+        if (s == 1 || cost < best) { split = s; best = cost; }
+    }
     if (tiles * split > 0x7fffffffLL) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_gated: a result of %lld x %lld elements is too large", (long long)p.M, (long long)p.N);
     NK_CUDA(ctx, cudaFuncSetAttribute(nk_gated_dmma_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, GD_SMEM));
     cudaLaunchConfig_t cfg;

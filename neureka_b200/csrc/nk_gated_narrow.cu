@@ -5,10 +5,11 @@
 //
 // The weights are the product's A operand: 128 columns n are the rows of the tensor core's tile, the tokens (padded to 16, 32 or 64) its columns.
 // A 3xTF32 product needs hi and lo of every weight; writing them to memory and reading them back would move five times the weights' bytes
-// (nk_gated_tc.cu does, where a panel is used by many tiles). Here a warp brings 32 columns x 16 k into shared memory (cp.async, three or four
+// (nk_gated_tc.cu does, where a panel is used by many tiles). Here a warp brings 32 columns x 16 k into shared memory (cp.async, two or three
 // such patches ahead: loads into registers, two ahead, left the memory at a third of its rate), splits them in registers and stores hi
 // and lo into tensor memory, from where tcgen05.mma takes its A operand. The tokens' panels are split before (they are small) and come by TMA.
-// What is left is the stream of weights: 4 bytes per element against 6 multiply-adds per token.
+// What is left is the stream of weights: 4 bytes per element against 6 multiply-adds per token. 16 tokens x 4096 x 8192 69 us, where the weights' bytes take
+// 41; 64 tokens 85; 24 x 2048 x 5461 37 us (14): bound by the issue of the converters (split, store) and, from 64 tokens on, by the products.
 //
 // Roles, 18 warps: 0..15 converters in two groups, warp 16 fetches the tokens' panels, warp 17 issues the products. A stage is 32 k of both weights
 // (SUM: 64 k of one); every converter splits 32 columns x 16 k of it, warp w for lanes 32 (w % 4) of the tile. Tensor memory: three (two)

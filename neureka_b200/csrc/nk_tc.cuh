@@ -17,7 +17,7 @@
 //
 // Accumulation. The tensor core adds each product block into the accumulator with truncation (measured: a sum of K
 // same-signed terms came out low by K/8 * 3 * 2^-25 relative, 9e-5 at K = 8192). A tile's sum over k is therefore cut
-// into chunks of 128 k (48 accumulations, bias below 1.5e-6): the two accumulators alternate chunk by chunk, and the
+// into chunks of 128 k (48 accumulations, bias below 1.5e-6; a caller may ask for shorter ones): the two accumulators alternate chunk by chunk, and the
 // sixteen epilogue warps add every finished chunk into per-thread F32 running sums with ordinary round-to-nearest adds
 // while the next chunk's products already run into the other accumulator. The running sums of a tile (a quarter of its
 // columns per thread) go to the drain after its last chunk.
