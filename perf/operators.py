@@ -180,29 +180,27 @@ def _gated_plain(s, train):
 
 
 # ---- the framework's operators -----------------------------------------------------------------------------------
-def _wrapped(device, values):
+class _Wrapped:
     """the C ABI's handle of a program's own device memory and its view descriptor; freed with the object"""
-    import ctypes as C
-    from neureka_b200 import _lib as L
-    from neureka_b200.ndconf import NDConfiguration
 
-    class Buffer:
-        def __init__(self):
-            self.handle = C.c_void_p()
-            L.check(L.lib.nk_wrap(device.ctx, L.NK_F32 if values.dtype == torch.float32 else L.NK_F64, C.c_void_p(values.data_ptr()), values.numel(),
-                                  C.byref(self.handle)), device.ctx)
-            self.values = values
-            self.conf = NDConfiguration.of_shape(tuple(values.shape))
-            self.describe(self.conf)
+    def __init__(self, device, values):
+        import ctypes as C
+        from neureka_b200 import _lib as L
+        from neureka_b200.ndconf import NDConfiguration
+        self.device, self.values, self.handle = device, values, C.c_void_p()
+        L.check(L.lib.nk_wrap(device.ctx, L.NK_F32 if values.dtype == torch.float32 else L.NK_F64, C.c_void_p(values.data_ptr()), values.numel(),
+                              C.byref(self.handle)), device.ctx)
+        self.conf = NDConfiguration.of_shape(tuple(values.shape))
+        self.describe(self.conf)
 
-        def describe(self, conf):
-            self._inline = conf.as_inline_array()
-            self.cfg = self._inline.ctypes.data_as(C.POINTER(C.c_int32))
+    def describe(self, conf):
+        import ctypes as C
+        self._inline = conf.as_inline_array()
+        self.cfg = self._inline.ctypes.data_as(C.POINTER(C.c_int32))
 
-        def __del__(self):
-            L.lib.nk_free(device.ctx, self.handle)
-
-    return Buffer()
+    def __del__(self):
+        from neureka_b200 import _lib as L
+        L.lib.nk_free(self.device.ctx, self.handle)
 
 
 def _tensor(device, values):
@@ -237,7 +235,7 @@ def _held(s):
     if "held" not in s:
         from neureka_b200.device import CudaDevice
         device = CudaDevice.get(0)
-        make = _tensor if s["case"]["train"] else _wrapped
+        make = _tensor if s["case"]["train"] else _Wrapped
         held = {k: make(device, v) for k, v in s.items() if isinstance(v, torch.Tensor)}
         held["device"] = device
         turned = s["case"].get("turned", False)
