@@ -186,24 +186,23 @@ def extreme(x: Tensor, want_max: bool) -> Tensor:
     return out
 
 
-class _Joint:
-    """The errors of an operation's operands that one kernel call computes together: made when the backward pass asks for the first one,
-    handed out one after the other, gone with the last."""
+def _joint(operands, compute: Callable[[Tensor, List[bool]], List[Optional[Tensor]]]) -> List[Tuple[Tensor, Callable[[Tensor], Tensor]]]:
+    """The parents of a node whose operands' errors one kernel call computes together: made when the backward pass asks for the first
+    one, handed out one after the other, gone with the last. Nothing that the actions hold leads back to them: a cycle would keep the operands
+    and what the forward call left for the backward pass until the interpreter's cycle collector happened to run."""
+    wanted = [t is not None and _tracks(t) for t in operands]
+    indices = [i for i, w in enumerate(wanted) if w]
+    ready: List[Optional[Tensor]] = []
 
-    def __init__(self, operands, compute: Callable[[Tensor, List[bool]], List[Optional[Tensor]]]):
-        self._wanted = [t is not None and _tracks(t) for t in operands]
-        self._compute = compute
-        self._ready: List[Optional[Tensor]] = []
-        indices = [i for i, w in enumerate(self._wanted) if w]
-        self.parents = [(operands[i], lambda err, i=i: self._take(i, err, i == indices[0], i == indices[-1])) for i in indices]
-
-    def _take(self, i: int, err: Tensor, first: bool, last: bool) -> Tensor:
-        if first:
-            self._ready = self._compute(err, self._wanted)
-        e = self._ready[i]
-        if last:
-            self._ready = []
+    def take(i: int, err: Tensor) -> Tensor:
+        if i == indices[0]:
+            ready[:] = compute(err, wanted)
+        e = ready[i]
+        if i == indices[-1]:
+            ready.clear()
         return e
+
+    return [(operands[i], lambda err, i=i: take(i, err)) for i in indices]
 
 
 def layer_norm(x: Tensor, gain: Optional[Tensor], shift: Optional[Tensor], eps: float) -> Tensor:
@@ -211,8 +210,7 @@ def layer_norm(x: Tensor, gain: Optional[Tensor], shift: Optional[Tensor], eps: 
     out, stats = F.run_layer_norm(x, gain, shift, eps, tracked)
     if tracked:
         stats.is_intermediate = False
-        joint = _Joint((x, gain, shift), lambda err, wanted: F.run_layer_norm_gradients(err, x, gain, shift, stats, wanted))
-        out.graph_node = GraphNode(out, joint.parents)
+        out.graph_node = GraphNode(out, _joint((x, gain, shift), lambda err, wanted: F.run_layer_norm_gradients(err, x, gain, shift, stats, wanted)))
     return out
 
 
@@ -233,8 +231,7 @@ def gated(x: Tensor, w_gate: Tensor, w_up: Tensor, fun: str) -> Tensor:
     out, kept = F.run_gated(x, w_gate, w_up, fun, tracked)
     if tracked:
         kept.is_intermediate = False
-        joint = _Joint((x, w_gate, w_up), lambda err, wanted: F.run_gated_gradients(err, x, w_gate, w_up, kept, fun, wanted))
-        out.graph_node = GraphNode(out, joint.parents)
+        out.graph_node = GraphNode(out, _joint((x, w_gate, w_up), lambda err, wanted: F.run_gated_gradients(err, x, w_gate, w_up, kept, fun, wanted)))
     return out
 
 

@@ -101,3 +101,38 @@ def test_vectors_of_any_view_are_described_with_one_dim():
         shape, strides, indices_map, offset, spread = (at[i] for i in range(5))
         flat = ND((shape,), (strides,), (indices_map,), (spread,), (offset,))
         assert flat.element_offsets().tolist() == t.ndconf.element_offsets().tolist()
+
+
+@pytest.mark.parametrize("through", [False, True])
+def test_a_node_lets_go_of_what_it_kept_with_its_last_reference(monkeypatch, through):
+    """The operands, the statistics and the kept products of a step go with its result, not with the next run of the cycle collector."""
+    import gc
+    import weakref
+    from neureka_b200 import functions as F
+    from neureka_b200.tensor import Tensor
+
+    def tensor(*shape):
+        return Tensor.of(np.float32, shape, np.zeros(int(np.prod(shape))))
+
+    def made(t):
+        seen.append(weakref.ref(t))
+        return t
+    seen = []
+    monkeypatch.setattr(F, "run_layer_norm", lambda x, gain, shift, eps, keep: (made(tensor(2, 3)), made(tensor(2, 2))))
+    monkeypatch.setattr(F, "run_gated", lambda x, w_gate, w_up, fun, keep: (made(tensor(2, 5)), made(tensor(2, 2, 5))))
+    monkeypatch.setattr(F, "run_layer_norm_gradients", lambda err, x, gain, shift, stats, wanted: [made(tensor(2, 3)), made(tensor(3)), made(tensor(3))])
+    monkeypatch.setattr(F, "run_gated_gradients", lambda err, x, w_gate, w_up, kept, fun, wanted: [made(tensor(2, 3)), made(tensor(3, 5)), made(tensor(3, 5))])
+    gc.collect()
+    gc.disable()
+    try:
+        x, gain, shift, w_gate, w_up = (made(tensor(*s).set_rqs_gradient(True)) for s in ((2, 3), (3,), (3,), (3, 5), (3, 5)))
+        y = x.layer_norm(gain, shift).gated(w_gate, w_up)
+        if through:   # what the backward pass does with a node's parents
+            errors = [act(y) for _, act in y.graph_node.parents]
+            errors += [act(errors[0]) for _, act in y.graph_node.parents[0][0].graph_node.parents]
+            assert [e.shape for e in errors] == [(2, 3), (3, 5), (3, 5), (2, 3), (3,), (3,)]
+            del errors
+        del x, gain, shift, w_gate, w_up, y
+        assert [r for r in seen if r() is not None] == []
+    finally:
+        gc.enable()
