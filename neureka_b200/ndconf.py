@@ -100,6 +100,11 @@ class NDConfiguration:
         """as_inline_array for a call of the library: a pointer to its ints, which live as long as the configuration."""
         return self.as_inline_array().ctypes.data_as(C.POINTER(C.c_int32))
 
+    def __getstate__(self):
+        """What copies and pickles of a configuration carry: its fields, and not what has been worked out from them (a pointer means
+        nothing elsewhere)."""
+        return {f: self.__dict__[f] for f in self.__dataclass_fields__}
+
     def is_compact(self) -> bool:
         """isCompact (NDConfiguration.java:386-392)."""
         return self._compact

@@ -136,3 +136,18 @@ def test_a_node_lets_go_of_what_it_kept_with_its_last_reference(monkeypatch, thr
         assert [r for r in seen if r() is not None] == []
     finally:
         gc.enable()
+
+
+def test_a_configuration_that_served_a_call_can_be_copied_and_pickled():
+    import copy
+    import pickle
+    from neureka_b200.ndconf import NDConfiguration as ND
+    from neureka_b200.tensor import Tensor
+    t = Tensor.of(np.float32, [4, 6], np.arange(24))
+    for c in (ND.of_shape((2, 3)), ND.virtual_of((5,)), t.ndconf, ND.of_shape((4, 6)).sliced([2, 3], [1, 0], [1, 2])):
+        before = c.inline_pointer[0], c.rank, c.size, c.is_compact()
+        for other in (pickle.loads(pickle.dumps(c)), copy.deepcopy(c), copy.copy(c)):
+            assert other == c and hash(other) == hash(c)
+            assert (other.inline_pointer[0], other.rank, other.size, other.is_compact()) == before
+            assert [other.inline_pointer[i] for i in range(5 * c.rank)] == c.as_inline_array().tolist()
+    assert np.array_equal(copy.deepcopy(t).numpy(), t.numpy())
