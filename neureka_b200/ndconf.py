@@ -72,12 +72,12 @@ class NDConfiguration:
     @staticmethod
     def of_shape(shape, layout: Layout = Layout.ROW_MAJOR) -> "NDConfiguration":
         """The configuration of a freshly created tensor (NDConstructor: row-major strides and indicesMap)."""
-        return _of_shape(shape if type(shape) is tuple else tuple(shape), layout)
+        return _shared(_of_shape, shape, layout)
 
     @staticmethod
     def virtual_of(shape) -> "NDConfiguration":
         """VirtualNDConfiguration (ndim/config/types/views/virtual/VirtualNDConfiguration.java): one element stands for all."""
-        return _virtual_of(shape if type(shape) is tuple else tuple(shape))
+        return _shared(_virtual_of, shape)
 
     # ---- queries (a configuration never changes: what is asked for with every call is worked out once) -----
     @cached_property
@@ -194,6 +194,14 @@ class NDConfiguration:
 
 
 # A program makes tensors of the same few shapes over and over: their (immutable) configurations are shared.
+def _shared(make, shape, *rest) -> NDConfiguration:
+    shape = shape if type(shape) is tuple else tuple(shape)
+    try:
+        return make(shape, *rest)
+    except TypeError:   # extents that cannot be looked up as they are (arrays without dims)
+        return make(tuple(int(x) for x in shape), *rest)
+
+
 @lru_cache(maxsize=4096)
 def _of_shape(shape: Tuple[int, ...], layout: Layout) -> NDConfiguration:
     shape = tuple(int(x) for x in shape)

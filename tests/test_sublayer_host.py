@@ -151,3 +151,17 @@ def test_a_configuration_that_served_a_call_can_be_copied_and_pickled():
             assert (other.inline_pointer[0], other.rank, other.size, other.is_compact()) == before
             assert [other.inline_pointer[i] for i in range(5 * c.rank)] == c.as_inline_array().tolist()
     assert np.array_equal(copy.deepcopy(t).numpy(), t.numpy())
+
+
+def test_extents_of_any_kind_that_converts_to_a_number():
+    from neureka_b200.ndconf import Layout, NDConfiguration as ND
+    for shape in ((2, 3), [2, 3], (np.int64(2), np.int32(3)), (np.array(2), np.array(3)), [np.array(2), 3], iter((2, 3)), np.array([2, 3]), (2.0, 3.0)):
+        c = ND.of_shape(shape)
+        assert c.shape == (2, 3) and all(type(x) is int for x in c.shape) and c.strides == (3, 1)
+    assert ND.of_shape((np.array(2), 3), Layout.COLUMN_MAJOR) == ND.of_shape((2, 3), Layout.COLUMN_MAJOR)
+    assert ND.virtual_of((np.array(2), 3)) == ND.virtual_of([2, 3])
+    for shape in ((2, 0), (np.array(0),)):
+        with pytest.raises(ValueError, match="greater than 0"):
+            ND.of_shape(shape)
+    with pytest.raises(TypeError):
+        ND.of_shape((2, None))
