@@ -270,7 +270,7 @@ class CudaDevice:
         return self
 
     def has(self, tensor) -> bool:
-        data = tensor._data
+        data = getattr(tensor, "_data", None)   # (nothing, or no tensor at all, is not stored here)
         return isinstance(data, CudaData) and data.device is self and tensor.device is self
 
     contains = has

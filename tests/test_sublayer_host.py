@@ -165,3 +165,14 @@ def test_extents_of_any_kind_that_converts_to_a_number():
             ND.of_shape(shape)
     with pytest.raises(TypeError):
         ND.of_shape((2, None))
+
+
+def test_a_device_has_nothing_that_is_no_tensor():
+    from neureka_b200.device import CudaDevice
+    from neureka_b200.tensor import Tensor
+    device = object.__new__(CudaDevice)   # (none of these calls reaches the library)
+    for what in (None, "a", 3, [], Tensor.of(np.float32, [2], [1, 2])):
+        assert not device.has(what) and not device.contains(what)
+        with pytest.raises(ValueError, match="not stored on this device"):
+            device.restore(what)
+        assert device.free(what) is device
