@@ -4,7 +4,8 @@
 //   g = e * gain:  dx = r * (g - mean(g) - xh * mean(g * xh)),  dgain = sum over rows of e * xh,  dshift = sum over rows of e
 //
 // Every sum is taken in the tensor's type over a fixed partition of the row (or column), so the result does not depend on scheduling; v
-// comes from the differences to a mean that is known before (no difference of large sums).
+// comes from the differences to a mean that is known before (no difference of large sums). Where a row lies far from zero, what these
+// differences come to corrects the mean (norm_far, norm_settle).
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -110,6 +111,27 @@ __device__ __forceinline__ void norm_sum2(T& a, T& b, T (*smem)[THREADS / 32]) {
 #pragma unroll
     for (int w = 1; w < THREADS / 32; w++) { a += smem[0][w]; b += smem[1][w]; }
 }
+// A mean is off by some units in its last place (a sum was rounded on the way), and a row's result by that over its deviation: nothing where they are
+// alike, everything where the row is far from zero and narrow (a row of 1000.0 came out as -0.019 instead of 0). There the differences d to the
+// mean tell by how much: their sum is 0 for the true one. A row of equal values gets that value as its mean, whatever its length, since its
+// differences are exact and all the same. Every row would pay for one more sum (8192 x 8192: 92 us -> 102, 16384 x 4096 F64: 192 -> 212), so only rows
+// further from zero than four deviations do. The same answer in all threads that share mean and m2.
+template <class T>
+__device__ __forceinline__ bool norm_far(T mean, T v) {   // (asked after 1 / sqrt(v + eps) has been begun, which takes longer)
+    return mean * mean > T(16) * v;                       // (false for a NaN)
+}
+// the same value, of which the compiler does not know that: the differences taken above need not stay in registers for the rows that need them again (24 more
+// registers otherwise, which cost 200000 x 200 a third of its speed)
+__device__ __forceinline__ float norm_again(float v) { asm volatile("" : "+f"(v)); return v; }
+__device__ __forceinline__ double norm_again(double v) { asm volatile("" : "+d"(v)); return v; }
+// d: the sum of the differences to the mean
+template <class T>
+__device__ __forceinline__ void norm_settle(T& mean, T& rstd, T m2, T d, T n, T eps) {
+    const T by = d / n;
+    mean += by;
+    m2 -= d * by;
+    rstd = T(1) / sqrt((m2 > T(0) ? m2 / n : T(0)) + eps);
+}
 // (x - mean) * rstd * gain + shift for the vectors at c0 + (k * lanes + lane) * W, stored
 template <class T, int W, int NV>
 __device__ __forceinline__ void norm_results(T* y, const T* gain, const T* shift, const NormPlan& p, int64_t c0, int lane, int lanes, T mean, T rstd, T (&v)[NV][W]) {
@@ -132,11 +154,17 @@ __device__ __forceinline__ void norm_results(T* y, const T* gain, const T* shift
 
 // ---- rows that a group of lanes, a CTA or a cluster holds in registers ---------------------------------------------------------------
 // One pass over the data: x stays in registers between the mean, the variance and the result. Short rows, and calls with too few rows to keep teams
-// with rings busy (below), which the latency of a row bounds: 1 x 4096 5.4 us, 1000 x 777 forward 8.2 us; 400000 x 64 67 us (3.0 TB/s).
+// with rings busy (below), which the latency of a row bounds: 1 x 4096 5.4 us, 1000 x 777 forward 8.2 us; 400000 x 64 69 us (3.0 TB/s).
 
+// CTAs per SM that the registers have to leave room for: fewer cost more than a few spilled words (200000 x 200 by two of them 140 us, by three 109)
+template <class T, int W, int E>
+constexpr int norm_lanes_ctas() {
+    const bool wide = sizeof(T) == 8 && W > 1;
+    return E == 4 ? (wide ? 3 : 4) : E == 8 ? (wide ? 2 : 3) : (W == 1 && sizeof(T) == 4 ? 3 : 2);
+}
 // A row per group of G lanes, E elements per lane.
 template <class T, int W, int G, int E>
-__global__ void __launch_bounds__(256) nk_norm_lanes_kernel(T* out, const T* src, const T* __restrict__ gain, const T* __restrict__ shift, T* __restrict__ stats,
+__global__ void __launch_bounds__(256, norm_lanes_ctas<T, W, E>()) nk_norm_lanes_kernel(T* out, const T* src, const T* __restrict__ gain, const T* __restrict__ shift, T* __restrict__ stats,
                                                             const NormPlan p, T eps) {
     constexpr int NV = E / W;
     const int lane = threadIdx.x % G;
@@ -156,8 +184,7 @@ __global__ void __launch_bounds__(256) nk_norm_lanes_kernel(T* out, const T* src
             for (int j = 0; j < W; j++) sum += v[k][j];
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const T mean = sum / n;
-        T m2 = T(0);
+        T mean = sum / n, m2 = T(0);
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
@@ -165,7 +192,20 @@ __global__ void __launch_bounds__(256) nk_norm_lanes_kernel(T* out, const T* src
                 if ((k * G + lane) * W + j < p.n) m2 += (v[k][j] - mean) * (v[k][j] - mean);
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
-        const T rstd = T(1) / sqrt(m2 / n + eps);
+        const T v2 = m2 / n;
+        T rstd = T(1) / sqrt(v2 + eps);
+        if (__any_sync(0xffffffffu, norm_far(mean, v2))) {
+            const T from = norm_again(mean);
+            T off = T(0);
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int j = 0; j < W; j++)
+                    if ((k * G + lane) * W + j < p.n) off += v[k][j] - from;
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) off += __shfl_xor_sync(0xffffffffu, off, o);
+            if (norm_far(mean, v2)) norm_settle(mean, rstd, m2, off, n, eps);   // (a row's result does not depend on its neighbours)
+        }
         if (!mine) continue;
         if (stats && lane == 0) { stats[row] = mean; stats[p.rows + row] = rstd; }
         norm_results<T, W, NV>(out + norm_row<0>(p, row), gain, shift, p, int64_t(0), lane, G, mean, rstd, v);
@@ -176,7 +216,7 @@ template <class T, int W, int THREADS, int E>
 __global__ void __launch_bounds__(THREADS) nk_norm_cta_kernel(T* out, const T* src, const T* __restrict__ gain, const T* __restrict__ shift, T* __restrict__ stats,
                                                               const NormPlan p, T eps) {
     constexpr int NV = E / W;
-    __shared__ T warps[2][THREADS / 32], parts[2][2];
+    __shared__ T warps[3][THREADS / 32], parts[2][3];
     cg::cluster_group cluster = cg::this_cluster();
     const int size = int(cluster.num_blocks()), rank = int(cluster.block_rank());
     const int64_t c0 = int64_t(rank) * THREADS * E, step = gridDim.x / unsigned(size);
@@ -200,14 +240,25 @@ __global__ void __launch_bounds__(THREADS) nk_norm_cta_kernel(T* out, const T* s
         for (int k = 0; k < NV; k++)
 #pragma unroll
             for (int j = 0; j < W; j++) sum += v[k][j];
-        const T mean = total(sum, 0) / n;
-        T m2 = T(0);
+        T mean = total(sum, 0) / n, m2 = T(0);
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
             for (int j = 0; j < W; j++)
                 if (c0 + (k * THREADS + int(threadIdx.x)) * W + j < p.n) m2 += (v[k][j] - mean) * (v[k][j] - mean);
-        const T rstd = T(1) / sqrt(total(m2, 1) / n + eps);
+        m2 = total(m2, 1);
+        const T v2 = m2 / n;
+        T rstd = T(1) / sqrt(v2 + eps);
+        if (norm_far(mean, v2)) {
+            const T from = norm_again(mean);
+            T off = T(0);
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int j = 0; j < W; j++)
+                    if (c0 + (k * THREADS + int(threadIdx.x)) * W + j < p.n) off += v[k][j] - from;
+            norm_settle(mean, rstd, m2, total(off, 2), n, eps);
+        }
         if (stats && rank == 0 && threadIdx.x == 0) { stats[row] = mean; stats[p.rows + row] = rstd; }
         norm_results<T, W, NV>(out + norm_row<0>(p, row), gain, shift, p, c0, threadIdx.x, THREADS, mean, rstd, v);
     }
@@ -359,7 +410,7 @@ __global__ void __launch_bounds__(256) nk_norm_grad_lanes_kernel(T* out, const T
 // ---- many rows: one CTA per SM, rows fetched ahead by bulk copies --------------------------------------------------------------------
 // A team of TW warps takes a row at a time. Its rows arrive in shared memory by cp.async.bulk, several ahead, so that the memory is kept busy
 // through the reductions; the copies need nothing but 16-byte boundaries around a row, so rows that start anywhere cost no more than aligned ones
-// (element-wise loads of rows into registers reached a third of the memory's rate). Forward and backward: 16384 x 4096 99 and 153 us (5.4 and 5.3
+// (element-wise loads of rows into registers reached a third of the memory's rate). Forward and backward: 16384 x 4096 98 and 153 us (5.5 and 5.3
 // TB/s, bound by the memory), 8192 x 8192 92 / 162, 30000 x 1001 47 / 81; rows that a cluster shares wait for its slowest CTA: 2000 x 20000 162 / 227
 // (2 TB/s). A row's 16-byte boundaries may lie outside its buffer at
 // the buffer's ends: such a row is read by plain loads.
@@ -505,7 +556,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, 1) nk_norm_stream_kernel(T* ou
     extern __shared__ __align__(16) unsigned char stream_smem[];
     __shared__ uint64_t bars[TEAMS * STREAM_STAGES];
     __shared__ int places[TEAMS * STREAM_STAGES][1];
-    __shared__ T sums[2][TEAMS][TW][1], parts[2][2];
+    __shared__ T sums[3][TEAMS][TW][1], parts[2][3];
     cg::cluster_group cluster = cg::this_cluster();
     const int size = int(cluster.num_blocks());
     auto ring = stream_ring<T, TW, 1>(p, call, src, static_cast<const T*>(nullptr), stream_smem, bars, places);
@@ -559,7 +610,24 @@ __global__ void __launch_bounds__(STREAM_THREADS, 1) nk_norm_stream_kernel(T* ou
             mean = all;
             m2[0] = all2;
         }
-        const T rstd = T(1) / sqrt(m2[0] * inv_n + eps);
+        const T v2 = m2[0] * inv_n;
+        T rstd = T(1) / sqrt(v2 + eps);
+        if (norm_far(mean, v2)) {
+            const T from = norm_again(mean);
+            T off[1] = {T(0)};
+            NK_EACH(k) {
+#pragma unroll
+                for (int j = 0; j < W; j++) off[0] += v[k][j] - from;
+            }
+            team_sum<T, TW, 1>(off, sums[2][team], team);
+            if (size > 1) {
+                if (threadIdx.x == 0) parts[turn & 1][2] = off[0];
+                cluster.sync();
+                off[0] = T(0);
+                for (int r = 0; r < size; r++) off[0] += cluster.map_shared_rank(&parts[turn & 1][0], r)[2];
+            }
+            norm_settle(mean, rstd, m2[0], off[0], T(p.n), eps);
+        }
         if (stats && ring.c0 == 0 && ring.leader) { stats[row] = mean; stats[p.rows + row] = rstd; }
         T* y = out + norm_row<0>(p, row) + ring.c0 + c_lane;
         NK_EACH(k) {
@@ -690,18 +758,25 @@ __global__ void __launch_bounds__(NORM_THREADS) nk_norm_chunk_stats_kernel(const
 #pragma unroll
             for (int j = 0; j < W; j++) sum += v[k][j];
         }
-        const T mean = norm_cta_sum(sum, smem) / T(left);
-        T m2 = T(0);
+        T mean = norm_cta_sum(sum, smem) / T(left), m2 = T(0), off = T(0);
 #pragma unroll
         for (int k = 0; k < NORM_NV; k++)
 #pragma unroll
             for (int j = 0; j < W; j++)
-                if (c0 + (k * NORM_THREADS + threadIdx.x) * W + j < p.n) m2 += (v[k][j] - mean) * (v[k][j] - mean);
+                if (c0 + (k * NORM_THREADS + threadIdx.x) * W + j < p.n) {
+                    const T d = v[k][j] - mean;
+                    off += d;
+                    m2 += d * d;
+                }
+        off = norm_cta_sum(off, smem);   // (corrects the mean, as norm_settle does)
         m2 = norm_cta_sum(m2, smem);
+        const T by = off / T(left);
+        mean += by;
+        m2 = m2 - off * by > T(0) ? m2 - off * by : T(0);
         if (threadIdx.x == 0) { part[2 * u] = mean; part[2 * u + 1] = m2; }
     }
 }
-// The row's mean and variance from its chunks': mu = sum(n_i mean_i) / n, v = sum(m2_i + n_i (mean_i - mu)^2) / n; then the chunk's results.
+// The row's mean and variance from its chunks': mu = mean_0 + sum(n_i (mean_i - mean_0)) / n, v = sum(m2_i + n_i (mean_i - mu)^2) / n; then the chunk's results.
 template <class T, int W>
 __global__ void __launch_bounds__(NORM_THREADS) nk_norm_chunk_apply_kernel(T* out, const T* src, const T* __restrict__ part, const T* __restrict__ gain,
                                                                            const T* __restrict__ shift, T* __restrict__ stats, const NormPlan p, int64_t chunks, T eps) {
@@ -710,9 +785,10 @@ __global__ void __launch_bounds__(NORM_THREADS) nk_norm_chunk_apply_kernel(T* ou
     for (int64_t u = blockIdx.x; u < p.rows * chunks; u += gridDim.x) {
         const int64_t row = u / chunks, chunk = u - row * chunks, c0 = chunk * L;
         auto length = [&](int64_t i) { return T(i + 1 < chunks ? L : p.n - i * L); };
+        const T base = part[2 * row * chunks];
         T sum = T(0);
-        for (int64_t i = threadIdx.x; i < chunks; i += NORM_THREADS) sum += length(i) * part[2 * (row * chunks + i)];
-        const T mean = norm_cta_sum(sum, smem) / T(p.n);
+        for (int64_t i = threadIdx.x; i < chunks; i += NORM_THREADS) sum += length(i) * (part[2 * (row * chunks + i)] - base);
+        const T mean = base + norm_cta_sum(sum, smem) / T(p.n);
         T m2 = T(0);
         for (int64_t i = threadIdx.x; i < chunks; i += NORM_THREADS) {
             const T d = part[2 * (row * chunks + i)] - mean;

@@ -43,3 +43,38 @@ def test_a_step_gives_its_memory_back_with_the_last_reference(device, what, thro
             assert (device.number_of_data_objects(), device.number_of_stored()) == before
     finally:
         gc.enable()
+
+
+# ---- rounding that could carry something away ----------------------------------------------------------------------------------------
+# forms of the kernel: groups of lanes, a CTA, a cluster, rows fetched ahead (by one CTA, by a cluster), chunks
+CONSTANT = [(8, 1000), (5000, 96), (2500, 1000), (6000, 300), (1300, 2047), (700, 4096), (310, 12001), (80, 40004), (2, 20000), (3, 300007)]
+
+
+@pytest.mark.parametrize("shape", CONSTANT, ids=str)
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_layer_norm_of_a_constant_row_is_the_shift(device, dtype, shape):
+    """However many rows there are, and however small eps: the mean of equal values is that value."""
+    levels = np.array([3.0, 100.0, 1000.0, 0.1, 1000.1, -1e-3, 12345.678, 0.0], dtype=dtype)
+    x = np.repeat(levels[np.arange(shape[0]) % len(levels)][:, None], shape[1], 1)
+    gain, shift = np.linspace(0.5, 2, shape[1]).astype(dtype), np.linspace(-1, 1, shape[1]).astype(dtype)
+    for eps in (1e-5, 1e-12):
+        y = put(device, x).layer_norm(put(device, gain), put(device, shift), eps).numpy()
+        assert np.array_equal(y, np.repeat(shift[None], shape[0], 0)), np.abs(y - shift).max(1)[:8]
+
+
+@pytest.mark.parametrize("shape", [(6000, 300), (2500, 777), (5000, 64), (6000, 256), (700, 4096), (310, 12001), (160, 16384), (4, 1024), (2, 140001), (3, 262144)], ids=str)
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_layer_norm_column_sums_take_every_row_once(device, dtype, shape):
+    """An error of small integers: dshift is the integer sum itself. With rows of pairs of 1 and -1 (mean 0, variance 1) and eps 0, the normalised
+    values are 1 and -1 and dgain is an integer sum too."""
+    rng = np.random.default_rng(52)
+    rows, n = shape
+    x = np.ones(shape, dtype)
+    x[:, 1::2] = -1
+    x *= np.repeat(rng.choice([-1, 1], (rows, (n + 1) // 2)), 2, 1)[:, :n].astype(dtype)   # (pairs, so that parts of a row have mean 0 too)
+    e = rng.integers(-8, 9, shape).astype(dtype)
+    tx, gain, shift = put(device, x), put(device, np.ones(n, dtype)).set_rqs_gradient(True), put(device, np.zeros(n, dtype)).set_rqs_gradient(True)
+    tx.layer_norm(gain, shift, 0.0).backward(put(device, e))
+    assert np.array_equal(shift.gradient.numpy(), e.sum(0))
+    if n & (n - 1) == 0:   # (the variance is exactly 1)
+        assert np.array_equal(gain.gradient.numpy(), (e * x).sum(0))
