@@ -18,7 +18,10 @@ namespace cg = cooperative_groups;
 namespace {
 
 // ---- the tile kernel -------------------------------------------------------------------------------------------------------------
-// For what is too small to fill the chip: bound by latency (200 x 128 x 256 forward would be 20 us, on the tensor cores 16).
+// For what is too small for the tensor cores, or too narrow: bound by latency (200 x 128 x 256 forward would be 20 us, on the tensor cores 16).
+// One running sum of K terms of one sign is 2e-8 sqrt(K) off (standard deviation; 2e-5 for a million terms, more than a product of the framework may be),
+// and where the tiles are few and the sums long (dW of a narrow block: all tokens) the chip is idle. So k is split over the CTAs, and a second
+// launch adds the parts in order: backward pass of 65536 x 32 x 32 7350 -> 119 us.
 // FORWARD: C_i = A_0 B_i, out_0 = f(C_0) * C_1 (C_i kept where wanted).  TWO: out_i = A_0 B_i.  SUM: out_0 = A_0 B_0 + A_1 B_1.
 enum { GATED_FORWARD, GATED_TWO, GATED_SUM };
 struct GatedTile {
@@ -26,15 +29,40 @@ struct GatedTile {
     int64_t M, N, K;
     GatedMatrix a[2], b[2], out[2];   // [M, K], [K, N], [M, N]
     void *gate, *up;                  // FORWARD: row-major [M, N] or null
+    int splits;                       // parts that k is cut into; above 1 they go to
+    void* parts;                      // [part][product][M][N]
 };
 constexpr int GT = 64, GK = 16;       // 64 x 64 of out, panels of 16 k; 256 threads with 4 x 4 elements of each product
+constexpr int GT_LEAST = 32, GT_MOST = 256;   // panels of a part: at least so many that its way through memory costs little, at most 4096 terms
 
+// element (m, n) of what is asked for, from its product or products
 template <class T, int MODE>
+__device__ __forceinline__ void gated_tile_store(const GatedTile& p, int64_t m, int64_t n, T v0, T v1) {
+    if (MODE == GATED_FORWARD) {
+        if (p.gate) {
+            static_cast<T*>(p.gate)[m * p.N + n] = v0;
+            static_cast<T*>(p.up)[m * p.N + n] = v1;
+        }
+        static_cast<T*>(p.out[0].ptr)[m * p.out[0].rs + n * p.out[0].cs] = gate_fun<T>(p.fun, false, v0) * v1;
+    } else {
+        if (p.out[0].ptr) static_cast<T*>(p.out[0].ptr)[m * p.out[0].rs + n * p.out[0].cs] = v0;
+        if (MODE == GATED_TWO && p.out[1].ptr) static_cast<T*>(p.out[1].ptr)[m * p.out[1].rs + n * p.out[1].cs] = v1;
+    }
+}
+
+// SPLIT: a part of k per CTA (a form of its own: the split's arithmetic makes whole sums an eighth slower)
+template <class T, int MODE, bool SPLIT>
 __global__ void __launch_bounds__(256) nk_gated_tile_kernel(const GatedTile p) {
     constexpr int NB = MODE == GATED_SUM ? 1 : 2, PHASES = MODE == GATED_SUM ? 2 : 1;
     __shared__ T As[GK][GT + 1], Bs[NB][GK][GT + 1];
-    const int64_t tiles_n = (p.N + GT - 1) / GT;
-    const int64_t m0 = (blockIdx.x / tiles_n) * GT, n0 = (blockIdx.x % tiles_n) * GT;
+    const int64_t tiles_n = (p.N + GT - 1) / GT, tile = SPLIT ? blockIdx.x / unsigned(p.splits) : blockIdx.x, part = SPLIT ? blockIdx.x % unsigned(p.splits) : 0;
+    const int64_t m0 = (tile / tiles_n) * GT, n0 = (tile % tiles_n) * GT;
+    int64_t first = 0, last = 0;   // this CTA's share of the panels of 16 k, of both phases of a SUM one after the other
+    const int64_t phase_panels = SPLIT ? (p.K + GK - 1) / GK : 0;
+    if (SPLIT) {
+        first = part * (phase_panels * PHASES) / p.splits;
+        last = (part + 1) * (phase_panels * PHASES) / p.splits;
+    }
     const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
     T acc[NB][4][4];
 #pragma unroll
@@ -45,7 +73,9 @@ __global__ void __launch_bounds__(256) nk_gated_tile_kernel(const GatedTile p) {
             for (int j = 0; j < 4; j++) acc[b][i][j] = T(0);
     for (int phase = 0; phase < PHASES; phase++) {
         const GatedMatrix& A = p.a[phase];
-        for (int64_t k0 = 0; k0 < p.K; k0 += GK) {
+        const int64_t k_begin = SPLIT && first > phase * phase_panels ? (first - phase * phase_panels) * GK : 0;
+        const int64_t k_end = SPLIT && last - phase * phase_panels < phase_panels ? (last - phase * phase_panels) * GK : p.K;
+        for (int64_t k0 = k_begin; k0 < k_end; k0 += GK) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 4; i++) {   // lanes along the contiguous direction
@@ -86,19 +116,38 @@ __global__ void __launch_bounds__(256) nk_gated_tile_kernel(const GatedTile p) {
         for (int j = 0; j < 4; j++) {
             const int64_t n = n0 + tx + 16 * j;
             if (n >= p.N) continue;
-            if (MODE == GATED_FORWARD) {
-                if (p.gate) {
-                    static_cast<T*>(p.gate)[m * p.N + n] = acc[0][i][j];
-                    static_cast<T*>(p.up)[m * p.N + n] = acc[NB - 1][i][j];
-                }
-                static_cast<T*>(p.out[0].ptr)[m * p.out[0].rs + n * p.out[0].cs] = gate_fun<T>(p.fun, false, acc[0][i][j]) * acc[NB - 1][i][j];
-            } else {
+            if (SPLIT) {
 #pragma unroll
-                for (int b = 0; b < NB; b++)
-                    if (p.out[b].ptr) static_cast<T*>(p.out[b].ptr)[m * p.out[b].rs + n * p.out[b].cs] = acc[b][i][j];
-            }
+                for (int b = 0; b < NB; b++) static_cast<T*>(p.parts)[((part * NB + b) * p.M + m) * p.N + n] = acc[b][i][j];
+            } else gated_tile_store<T, MODE>(p, m, n, acc[0][i][j], acc[NB - 1][i][j]);
         }
     }
+}
+// The parts of split sums, in a fixed order: 32 elements per CTA, warp w takes the parts w, w + 8, ...
+template <class T, int MODE>
+__global__ void __launch_bounds__(256) nk_gated_join_kernel(const GatedTile p) {
+    constexpr int NB = MODE == GATED_SUM ? 1 : 2;
+    __shared__ T sums[NB][8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t size = p.M * p.N, e = int64_t(blockIdx.x) * 32 + lane;
+    T v[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) v[b] = T(0);
+    if (e < size) {
+#pragma unroll 4
+        for (int s = warp; s < p.splits; s += 8)
+#pragma unroll
+            for (int b = 0; b < NB; b++) v[b] += static_cast<const T*>(p.parts)[(int64_t(s) * NB + b) * size + e];
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++) sums[b][warp][lane] = v[b];
+    __syncthreads();
+    if (warp || e >= size) return;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int w = 1; w < 8; w++) v[b] += sums[b][w][lane];
+    gated_tile_store<T, MODE>(p, e / p.N, e % p.N, v[0], v[NB - 1]);
 }
 // ---- F64 on the FP64 matrix instructions -----------------------------------------------------------------------------------------
 // mma.m8n8k4, 64 x 64 tiles of four warps with 32 x 32 each (nk_conv_gemm.cu: why). With two B operands the tile is 32 columns of each product and
@@ -289,13 +338,28 @@ int launch_dmma(nk_ctx* ctx, const GatedTile& p) {
 }
 
 template <class T, int MODE>
-int launch_tiles(nk_ctx* ctx, const GatedTile& p) {
+int launch_tiles(nk_ctx* ctx, GatedTile p) {
     if constexpr (sizeof(T) == 8) return launch_dmma<MODE>(ctx, p);
     else {
-        const int64_t tiles = ((p.M + GT - 1) / GT) * ((p.N + GT - 1) / GT);
+        const int64_t tiles = ((p.M + GT - 1) / GT) * ((p.N + GT - 1) / GT), panels = (p.K + GK - 1) / GK * (MODE == GATED_SUM ? 2 : 1);
         if (tiles > 0x7fffffffLL) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_gated: a result of %lld x %lld elements is too large", (long long)p.M, (long long)p.N);
-        nk_gated_tile_kernel<T, MODE><<<unsigned(tiles), 256, 0, ctx->stream>>>(p);
-        return nk_after_launch(ctx, "nk_gated_tile_kernel");
+        int64_t splits = int64_t(ctx->prop.multiProcessorCount) * 2 / tiles;   // what fits the chip, two CTAs per SM
+        if (splits > panels / GT_LEAST) splits = panels / GT_LEAST;
+        if (splits < (panels + GT_MOST - 1) / GT_MOST) splits = (panels + GT_MOST - 1) / GT_MOST;
+        if (tiles * splits > 0x7fffffffLL) return nk_fail(ctx, NK_ERR_UNSUPPORTED, "nk_gated: sums of %lld terms are too long", (long long)p.K);
+        p.splits = int(splits);
+        NkWorkspace ws(ctx);
+        int st;
+        if (p.splits > 1 && (st = ws.get(size_t(p.splits) * (MODE == GATED_SUM ? 1 : 2) * p.M * p.N * sizeof(T)))) return st;
+        p.parts = ws.ptr;
+        if (p.splits == 1) {
+            nk_gated_tile_kernel<T, MODE, false><<<unsigned(tiles), 256, 0, ctx->stream>>>(p);
+            return nk_after_launch(ctx, "nk_gated_tile_kernel");
+        }
+        nk_gated_tile_kernel<T, MODE, true><<<unsigned(tiles * p.splits), 256, 0, ctx->stream>>>(p);
+        if ((st = nk_after_launch(ctx, "nk_gated_tile_kernel"))) return st;
+        nk_gated_join_kernel<T, MODE><<<unsigned((p.M * p.N + 31) / 32), 256, 0, ctx->stream>>>(p);
+        return nk_after_launch(ctx, "nk_gated_join_kernel");
     }
 }
 

@@ -78,3 +78,30 @@ def test_layer_norm_column_sums_take_every_row_once(device, dtype, shape):
     assert np.array_equal(shift.gradient.numpy(), e.sum(0))
     if n & (n - 1) == 0:   # (the variance is exactly 1)
         assert np.array_equal(gain.gradient.numpy(), (e * x).sum(0))
+
+
+LONG = [(1 << 21, 4, 4), (200000, 48, 48), (70000, 20, 100), (9, 400000, 12), (12, 14, 300000)]
+
+
+@pytest.mark.parametrize("size", LONG, ids=str)
+def test_gated_of_narrow_blocks_with_long_sums_of_one_sign(device, size):
+    """A block with a narrow side and very many tokens (or the other way round): nothing cancels, so what a running sum loses shows. Each product within the
+    framework's bound for a product, 1e-5 of sum |a||b|; what the gate's small products before it were off by comes on top."""
+    t, d, h = size
+    rng = np.random.default_rng(53)
+    x, wg, wu, e = (rng.uniform(0.5, 1.5, s).astype(np.float32) for s in ((t, d), (d, h), (d, h), (t, h)))
+    tx, tg, tu = (put(device, a).set_rqs_gradient(True) for a in (x, wg, wu))
+    y = tx.gated(tg, tu, "idy")
+    y.backward(put(device, e))
+    X, G, U, E = (a.astype(np.float64) for a in (x, wg, wu, e))
+    g, u = X @ G, X @ U
+    tol = 1e-5
+    assert (np.abs(y.numpy() / (g * u) - 1) < 2 * tol + 1e-6).all()
+    dg, du = E * u, E * g
+    for name, got, want in (("dx", tx, dg @ G.T + du @ U.T), ("dwg", tg, X.T @ dg), ("dwu", tu, X.T @ du)):
+        # dg and du follow from one product each: off by `tol` where that one is long, by d roundings where it is short
+        first = tol if d > 1000 else d * S.unit(np.float32)
+        off = np.abs(got.gradient.numpy() / want - 1).max()
+        assert off < tol + first + 4 * S.unit(np.float32), (name, off)
+    again = put(device, x).gated(put(device, wg), put(device, wu), "idy")
+    assert np.array_equal(again.numpy(), y.numpy())
