@@ -228,11 +228,11 @@ int split(nk_ctx* ctx, const TcSplit& sp) {
 }
 // Chunks of 128 k leave a result 1.8e-6 off (2-norm, normal operands; the accumulator truncates), chunks of 64 k 0.9e-6, whatever the length of the
 // sum; a sum of F32 multiply-adds is 2.7e-8 sqrt(K) off. So sums of up to 4096 take the shorter chunks, which cost a tenth of the time (accumulators
-// are read out twice as often, and a tile's stores hide behind half as much: 4096 x 2048 x 8192 forward 1.18 -> 1.30 ms), and longer ones lose
+// are read out twice as often, and a tile's stores hide behind half as much: 4096 x 2048 x 8192 forward 1.18 -> 1.30 ms, 2048 x 4096 x 2048 0.35 -> 0.37), and longer ones lose
 // nothing by the longer ones.
 template <class Drain>
 int product(nk_ctx* ctx, const TcShape& shape, int64_t Kp, const TcPanels& a, const TcPanels& b0, const TcPanels& b1, TcParams tp, const Drain& drain) {
-    if (Kp < 4096) tp.chunk = TC_KC / 2;
+    if (Kp <= 4096) tp.chunk = TC_KC / 2;
     const int st = shape.pair ? tc_launch<2, 256>(ctx, "nk_conv_tc_kernel<3xtf32,pair>", Kp, a, b0, b1, tp, drain)
                               : tc_launch<1, 128>(ctx, "nk_conv_tc_kernel<3xtf32>", Kp, a, b0, b1, tp, drain);
     return st == -1 ? nk_fail(ctx, NK_ERR_CUDA, "nk_gated: the driver has no tensor-map encoder") : st;

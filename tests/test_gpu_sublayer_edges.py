@@ -105,3 +105,16 @@ def test_gated_of_narrow_blocks_with_long_sums_of_one_sign(device, size):
         assert off < tol + first + 4 * S.unit(np.float32), (name, off)
     again = put(device, x).gated(put(device, wg), put(device, wu), "idy")
     assert np.array_equal(again.numpy(), y.numpy())
+
+
+def test_gated_sums_of_4096_terms_take_the_short_accumulation_chunks(device):
+    """The tensor core truncates when it accumulates. n = 3 c / 8 accumulations in a chunk of c terms of one sign lose half a unit in the last place of a growing
+    partial sum each: the sum over i of 0.5 * 0.72 * 2^-23 * i / n (0.72: a unit in the last place over 2^-23 of the value, on average), 5e-7 for 64
+    terms and 10e-7 for 128. The mean over many sums shows which it was."""
+    rng = np.random.default_rng(54)
+    x, w, one = rng.uniform(0.5, 1.5, (256, 4096)).astype(np.float32), rng.uniform(0.5, 1.5, (4096, 256)).astype(np.float32), np.zeros((4096, 256), np.float32)
+    one[0] = 1
+    x[:, 0] = 1
+    y = put(device, x).gated(put(device, one), put(device, w), "idy").numpy()   # 1 * (x @ w)
+    want = x.astype(np.float64) @ w.astype(np.float64)
+    assert abs((y / want - 1).mean()) < 7e-7
