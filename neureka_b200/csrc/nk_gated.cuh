@@ -1,5 +1,5 @@
 // The gated feed-forward block: what the kernel families behind nk_gated / nk_gated_grad share.
-// f and f' are the framework's functions: F64 as they are (nk_scalarfun.cuh: the units are compiled with -fmad=false, products say fma), F32 below.
+// f and f' are the framework's functions (nk_scalarfun.cuh: the units are compiled with -fmad=false, products say fma).
 #pragma once
 #include "nk_internal.h"
 #include "nk_scalarfun.cuh"
@@ -21,9 +21,37 @@ struct GatedCall {
     GatedMatrix dx, dw[2];    // backward
 };
 
-// The sigmoid in F32 and what is left to 1, from e^-|x| <= 1, so that neither cancels: some 4 units in the last place. The framework's F32
-// functions evaluate it in F64 to be right to the last bit; here x is a product that is off by more than that, and at 64 F64 operations a clock an
-// epilogue of 128 x 128 of them took 15,000 cycles, twice as long as the next products hide: 4096 x 2048 x 8192 forward 1.48 -> 1.30 ms.
+// f(x) and f'(x). In F32 both are evaluated in F64 and rounded once: sig, silu, gelu, relu and idy are the framework's own values to the last bit; tanh and the
+// derivatives too are right to the last bit, where the framework's formulas (the reference's: 1 - s, 2 / (1 + e) - 1) cancel.
+__device__ __forceinline__ float gate_derivative(int f, float x) {
+    const double a = (f == NK_FUN_GELU ? 1.702 : f == NK_FUN_TANH ? 2.0 : 1.0) * double(x), c = fmin(fmax(a, -700.0), 700.0);   // (beyond, e and its products are 0 in F32)
+    const double e = nkf::nk_exp_reduced(-fabs(c)), t = 1.0 / (1.0 + e), both = e * t * t;   // both: s (1 - s)
+    const double v = f == NK_FUN_SIG ? both : f == NK_FUN_TANH ? 4.0 * both : (c < 0.0 ? e * t : t) + c * both;
+    return x != x ? x : float(v);
+}
+template <class T>
+__device__ __forceinline__ T gate_fun(int f, bool derive, T x) {
+    if constexpr (sizeof(T) == 4) {
+        if (f != NK_FUN_RELU && f != NK_FUN_IDY) {
+            if (derive) return gate_derivative(f, x);
+            if (f == NK_FUN_TANH) return float(tanh(double(x)));
+        }
+    }
+    switch (f) {
+        case NK_FUN_SIG: return nkf::fun(NK_FUN_SIG, derive, x);
+        case NK_FUN_SILU: return nkf::fun(NK_FUN_SILU, derive, x);
+        case NK_FUN_GELU: return nkf::fun(NK_FUN_GELU, derive, x);
+        case NK_FUN_RELU: return nkf::fun(NK_FUN_RELU, derive, x);
+        case NK_FUN_TANH: return nkf::fun(NK_FUN_TANH, derive, x);
+        default: return nkf::fun(NK_FUN_IDY, derive, x);
+    }
+}
+
+// The same in F32, where the products come from the tensor cores: the sigmoid and what is left to 1 from e^-|x| <= 1, so that neither cancels, some 4
+// units in the last place off, and x is a product that is off by more than that. At 64 F64 operations a clock an epilogue of 128 x 128 gates took 15,000
+// cycles, twice as long as the next products hide (4096 x 2048 x 8192 forward 1.48 -> 1.30 ms), and that of some tokens, which nothing hides, a
+// tenth of a small call (24 x 515 x 900 22.5 us, so 20.5). Where the products are F32 or F64 multiply-adds, memory or latency leaves room
+// for gate_fun (1 x 2048 x 5461 26.6 us against 25.6, 300 x 30 x 500 13.0 against 11.3).
 __device__ __forceinline__ float gate_sig(float x, float* rest) {
     const float e = expf(-fabsf(x)), t = __fdividef(1.0f, 1.0f + e), m = e * t;
     *rest = x < 0.0f ? t : m;
@@ -48,25 +76,14 @@ __device__ __forceinline__ float gate_fun32(int f, bool derive, float x) {
     if (f == NK_FUN_SIG) return derive ? s * rest : s;
     return derive ? fmaf(fminf(fmaxf(a, -128.0f), 128.0f) * rest, s, s) : x * s;   // (rest or s is 0 beyond, and 1.702 x may be infinite)
 }
-template <class T>
-__device__ __forceinline__ T gate_fun(int f, bool derive, T x) {
-    if constexpr (sizeof(T) == 4) {
-        switch (f) {
-            case NK_FUN_SIG: return gate_fun32(NK_FUN_SIG, derive, x);
-            case NK_FUN_SILU: return gate_fun32(NK_FUN_SILU, derive, x);
-            case NK_FUN_GELU: return gate_fun32(NK_FUN_GELU, derive, x);
-            case NK_FUN_RELU: return gate_fun32(NK_FUN_RELU, derive, x);
-            case NK_FUN_TANH: return gate_fun32(NK_FUN_TANH, derive, x);
-            default: return gate_fun32(NK_FUN_IDY, derive, x);
-        }
-    }
+__device__ __forceinline__ float gate_fun32(int f, float x) {   // of a call's function
     switch (f) {
-        case NK_FUN_SIG: return nkf::fun(NK_FUN_SIG, derive, x);
-        case NK_FUN_SILU: return nkf::fun(NK_FUN_SILU, derive, x);
-        case NK_FUN_GELU: return nkf::fun(NK_FUN_GELU, derive, x);
-        case NK_FUN_RELU: return nkf::fun(NK_FUN_RELU, derive, x);
-        case NK_FUN_TANH: return nkf::fun(NK_FUN_TANH, derive, x);
-        default: return nkf::fun(NK_FUN_IDY, derive, x);
+        case NK_FUN_SIG: return gate_fun32(NK_FUN_SIG, false, x);
+        case NK_FUN_SILU: return gate_fun32(NK_FUN_SILU, false, x);
+        case NK_FUN_GELU: return gate_fun32(NK_FUN_GELU, false, x);
+        case NK_FUN_RELU: return gate_fun32(NK_FUN_RELU, false, x);
+        case NK_FUN_TANH: return gate_fun32(NK_FUN_TANH, false, x);
+        default: return gate_fun32(NK_FUN_IDY, false, x);
     }
 }
 // CASE(FUN) for the function of a call

@@ -405,7 +405,7 @@ nk_gated_narrow_kernel(const __grid_constant__ CUtensorMap map_hi, const __grid_
 #pragma unroll 1
                     for (int j = 0; j < 4 && n + j < p.N; j++) {
                         const float v0 = res[e + j], v1 = SUM ? 0.0f : res[C::RES / 2 + e + j];
-                        o[j * p.out.cs] = SUM ? v0 : gate_fun<float>(p.fun, false, v0) * v1;
+                        o[j * p.out.cs] = SUM ? v0 : gate_fun32(p.fun, v0) * v1;
                         if (!SUM && p.gate) { p.gate[t * p.N + n + j] = v0; p.up[t * p.N + n + j] = v1; }
                     }
                 }

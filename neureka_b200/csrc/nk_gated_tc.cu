@@ -67,7 +67,7 @@ struct GatedDrain {
         for (int j = 0; j < HC; j += 16) {
             float v[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = gate_fun<float>(FUN, false, sum[j + i]) * sum[HC + j + i];
+            for (int i = 0; i < 16; i++) v[i] = gate_fun32(FUN, false, sum[j + i]) * sum[HC + j + i];
             store16(y, rs, cs, vec, m, n0 + j, M, N, v);
         }
         if (!gate) return;
@@ -163,8 +163,8 @@ __global__ void __launch_bounds__(256) nk_gated_errors_split_kernel(const GatedC
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            d[0][j] = e[j] * u[j] * gate_fun<float>(FUN, true, g[j]);
-            d[1][j] = e[j] * gate_fun<float>(FUN, false, g[j]);
+            d[0][j] = e[j] * u[j] * gate_fun32(FUN, true, g[j]);
+            d[1][j] = e[j] * gate_fun32(FUN, false, g[j]);
 #pragma unroll
             for (int b = 0; b < 2; b++) tile[b][warp + 8 * i][lane * 4 + j] = d[b][j];
         }

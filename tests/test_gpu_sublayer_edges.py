@@ -6,6 +6,8 @@ import numpy as np
 import pytest
 
 import sublayer as S
+from neureka_b200 import _lib as L
+from neureka_b200 import functions as F
 from test_gpu_sublayer import put
 
 pytestmark = pytest.mark.gpu
@@ -118,3 +120,47 @@ def test_gated_sums_of_4096_terms_take_the_short_accumulation_chunks(device):
     y = put(device, x).gated(put(device, one), put(device, w), "idy").numpy()   # 1 * (x @ w)
     want = x.astype(np.float64) @ w.astype(np.float64)
     assert abs((y / want - 1).mean()) < 7e-7
+
+
+@pytest.mark.parametrize("fun", L.GATES)
+def test_gates_of_plain_products_are_right_to_the_last_bit(device, fun):
+    """Where the products are F32 multiply-adds, sig, silu, gelu, relu and idy are the very values of the framework's functions, and tanh and all derivatives
+    the true ones rounded once from F64 (half a unit in the last place; what F64 was off by, and denormals, on top). x = [v, 1] with weights [1, 0] and
+    [0, 1] gives g = v, u = 1, y = f(v) and, for an error of ones, dx = [f'(v), f(v)]; tokens of [1, 1] with rows of v and ones the same for many columns."""
+    v = np.concatenate([np.linspace(-20, 20, 4001), np.linspace(-120, 120, 999), np.geomspace(1e-30, 3e38, 400), -np.geomspace(1e-30, 3e38, 400)]).astype(np.float32)
+    w, k = v.astype(S.WIDE), S.WIDE({"gelu": 1.702, "tanh": 2}.get(fun, 1))
+    e = np.exp(-k * np.abs(w))
+    s, rest = np.where(w < 0, e, 1) / (1 + e), np.where(w < 0, 1, e) / (1 + e)
+    if fun == "tanh":
+        f = np.tanh(w)
+    else:
+        f = F.run_function(fun, put(device, v)).numpy()
+    df = {"idy": lambda: np.ones_like(w), "relu": lambda: np.where(w >= 0, np.float32(1), np.float32(0.01)), "tanh": lambda: 4 * s * rest, "sig": lambda: s * rest}.get(
+        fun, lambda: s + k * w * s * rest)()
+
+    def same(got, want, what):
+        if want.dtype == np.float32:
+            assert np.array_equal(got, want), what
+        else:   # 2^-46: some hundred units in the last place of F64, relative to the terms, which a derivative's sum may cancel
+            bound = S.unit(np.float32) * np.abs(want) + 2.0 ** -46 * (np.abs(want) + s + np.abs(k * w) * s * rest) + 2.0 ** -149
+            S.assert_within(got, (want, bound), what)
+
+    column = [put(device, np.array(c, np.float32)) for c in ([[1], [0]], [[0], [1]])]
+    tx = put(device, np.stack([v, np.ones_like(v)], 1)).set_rqs_gradient(True)
+    y = tx.gated(*column, fun)
+    y.backward()
+    same(y.numpy()[:, 0], f, "f")
+    same(tx.gradient.numpy()[:, 1], f, "f again")
+    same(tx.gradient.numpy()[:, 0], df, "f'")
+    zero, one = np.zeros_like(v), np.ones_like(v)
+    for t in (1, 3, 8):
+        x = np.ones((t, 2), np.float32)
+        rows = [put(device, np.stack(r)).set_rqs_gradient(True) for r in ((v, zero), (zero, one))]
+        y = put(device, x).gated(*rows, fun)
+        y.backward()
+        for i in range(t):
+            same(y.numpy()[i], f, f"f of token {i}")
+        if t == 1:   # dWg = x^T (u f'(g)), dWu = x^T f(g)
+            for i in range(2):
+                same(rows[0].gradient.numpy()[i], df, "dWg")
+                same(rows[1].gradient.numpy()[i], f, "dWu")
