@@ -16,7 +16,8 @@
 // stages of 128 columns (4 x (16 hi + 16 lo)) and the accumulators. (Stages of half that size: the issuing warp's waits took as long as its products.)
 // A product of 128 x up to 128 x 8 takes about 86 cycles here whatever its width, so the tokens' hi and lo panels lie side by side as one operand:
 // hi x [hi | lo], then lo x hi onto the second half -- two products per 8 k instead of three, and the small terms have an accumulator of
-// their own. The tensor core truncates when it accumulates (nk_tc.cuh): the accumulators are read out every 256 k (32 accumulations) and added
+// their own. The tensor core truncates when it accumulates (nk_tc.cuh): the accumulators are read out every 256 k (32 accumulations), in small
+// calls every 64 (gated_small; 24 x 515 x 900 20.5 -> 22.5 us, 16 x 4096 x 8192 would take 71 for 64), and added
 // up in shared memory, rounding to nearest; where tensor memory has room for two sets the products go on meanwhile.
 // Units of 32 k of all tiles form one sequence that the CTAs share evenly; a tile that several CTAs have a part of is finished by the last of
 // them to arrive, which adds the parts in order (nobody waits; the same bits every time).
@@ -36,6 +37,7 @@ struct NarrowCall {
     GatedMatrix out;           // [T, N]
     float *gate, *up;          // forward: row-major [T, N] or null
     int units, tiles_t, tiles;   // units of a tile (SUM: both weights'), tiles along the tokens, all tiles
+    int chunk;                 // units between two readings of the accumulators, at least 1
     int64_t total;             // units of all tiles
     int64_t Kq;                // SUM: columns of a panel per weight, a multiple of a unit
     float* parts;              // [CTA][2][NB][NT][128]
@@ -46,7 +48,6 @@ template <int NT, bool SUM>
 struct NarrowCfg {
     static constexpr int NB = SUM ? 1 : 2;
     static constexpr int UNIT = SUM ? 64 : 32;                    // k of a unit of work, which is a stage
-    static constexpr int CHUNK = 256 / UNIT;                      // units between two readings of the accumulators
     static constexpr int PANEL = NT * 64;                         // NT tokens x 16 k
     static constexpr int RING_BYTES = UNIT / 16 * 2 * PANEL;      // hi and lo of a stage's k
     static constexpr int RING = SUM && NT == 64 ? 3 : 4;
@@ -179,8 +180,8 @@ nk_gated_narrow_kernel(const __grid_constant__ CUtensorMap map_hi, const __grid_
         auto all_lanes = [&](bool mine) { return __all_sync(0xffffffffu, mine) != 0; };
         for (int first = 0, end; first < count && ok; first = end) {
             end = tile_end(first);
-            for (int from = first; from < end && ok; from += C::CHUNK, chunk++) {
-                const int to = from + C::CHUNK < end ? from + C::CHUNK : end;
+            for (int from = first; from < end && ok; from += p.chunk, chunk++) {
+                const int to = from + p.chunk < end ? from + p.chunk : end;
                 const unsigned set = C::SETS == 2 ? chunk & 1u : 0u, use = C::SETS == 2 ? chunk >> 1 : chunk;
                 ok = all_lanes(wait(&acc_free[set], (use & 1u) ^ 1u));
 #pragma unroll 1
@@ -418,8 +419,8 @@ nk_gated_narrow_kernel(const __grid_constant__ CUtensorMap map_hi, const __grid_
         bool before_fresh = false;
         for (int first = 0, end; first < count; first = end) {
             end = tile_end(first);
-            for (int from = first; from < end; from += C::CHUNK, chunk++) {
-                const int to = from + C::CHUNK < end ? from + C::CHUNK : end;
+            for (int from = first; from < end; from += p.chunk, chunk++) {
+                const int to = from + p.chunk < end ? from + p.chunk : end;
                 const int n = to - from, head = n < 2 ? n : 2;
                 convert(head);
                 if (chunk > 0) {
@@ -446,13 +447,14 @@ nk_gated_narrow_kernel(const __grid_constant__ CUtensorMap map_hi, const __grid_
 
 int narrow_tokens(int64_t T) { return T <= 16 ? 16 : T <= 32 ? 32 : 64; }
 int narrow_unit(bool sum) { return sum ? NarrowCfg<16, true>::UNIT : NarrowCfg<16, false>::UNIT; }
-void narrow_tiles(NarrowCall* p, bool sum) {
+void narrow_tiles(NarrowCall* p, bool sum, bool small) {
     const int64_t nt = narrow_tokens(p->T);
     const int64_t unit = narrow_unit(sum);
     p->units = int((p->K + unit - 1) / unit) * (sum ? 2 : 1);
     p->tiles_t = int((p->T + nt - 1) / nt);
     p->tiles = int((p->N + 127) / 128) * p->tiles_t;
     p->total = int64_t(p->tiles) * p->units;
+    p->chunk = int((small ? 64 : 256) / unit);
     p->Kq = (p->K + unit - 1) / unit * unit;
 }
 // at least four units per CTA: a tile's parts cost what there are of them
@@ -530,7 +532,7 @@ int nk_gated_narrow_forward(nk_ctx* ctx, const GatedCall& c) {
     p.gate = static_cast<float*>(c.gate);
     p.up = static_cast<float*>(c.up);
     p.status = ctx->tma_status_dev;
-    narrow_tiles(&p, false);
+    narrow_tiles(&p, false, gated_small(c));
     const int64_t Kp = tc_round_k(c.D);
     auto pad = [](size_t b) { return (b + 1023) / 1024 * 1024; };
     const size_t x_bytes = pad(size_t(c.T) * Kp * 4), part_bytes = pad(narrow_part_bytes(ctx, p, false));
@@ -563,7 +565,7 @@ static NarrowCall narrow_dx_call(nk_ctx* ctx, const GatedCall& c) {
     for (int b = 0; b < 2; b++) p.w[b] = GatedMatrix{c.w[b].ptr, c.w[b].cs, c.w[b].rs};
     p.out = c.dx;
     p.status = ctx->tma_status_dev;
-    narrow_tiles(&p, true);
+    narrow_tiles(&p, true, gated_small(c));
     return p;
 }
 void nk_gated_narrow_dx_needs(nk_ctx* ctx, const GatedCall& c, size_t* part_bytes, int* tickets) {

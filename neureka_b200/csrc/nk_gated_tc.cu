@@ -229,10 +229,11 @@ int split(nk_ctx* ctx, const TcSplit& sp) {
 // Chunks of 128 k leave a result 1.8e-6 off (2-norm, normal operands; the accumulator truncates), chunks of 64 k 0.9e-6, whatever the length of the
 // sum; a sum of F32 multiply-adds is 2.7e-8 sqrt(K) off. So sums of up to 4096 take the shorter chunks, which cost a tenth of the time (accumulators
 // are read out twice as often, and a tile's stores hide behind half as much: 4096 x 2048 x 8192 forward 1.18 -> 1.30 ms, 2048 x 4096 x 2048 0.35 -> 0.37), and longer ones lose
-// nothing by the longer ones.
+// nothing by the longer ones. Small calls take chunks of 32 (200 x 256 x 300 forward 20.5 -> 21.2 us, backward 48.8 -> 50.5).
 template <class Drain>
-int product(nk_ctx* ctx, const TcShape& shape, int64_t Kp, const TcPanels& a, const TcPanels& b0, const TcPanels& b1, TcParams tp, const Drain& drain) {
-    if (Kp <= 4096) tp.chunk = TC_KC / 2;
+int product(nk_ctx* ctx, const GatedCall& c, const TcShape& shape, int64_t Kp, const TcPanels& a, const TcPanels& b0, const TcPanels& b1, TcParams tp, const Drain& drain) {
+    if (gated_small(c)) tp.chunk = TC_KC / 4;
+    else if (Kp <= 4096) tp.chunk = TC_KC / 2;
     const int st = shape.pair ? tc_launch<2, 256>(ctx, "nk_conv_tc_kernel<3xtf32,pair>", Kp, a, b0, b1, tp, drain)
                               : tc_launch<1, 128>(ctx, "nk_conv_tc_kernel<3xtf32>", Kp, a, b0, b1, tp, drain);
     return st == -1 ? nk_fail(ctx, NK_ERR_CUDA, "nk_gated: the driver has no tensor-map encoder") : st;
@@ -273,7 +274,7 @@ int nk_gated_tc_forward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     const TcParams tp = tc_params(shape, c.T, Kp, at(parts), sp.tickets, ctx->tma_status_dev);
     const TcPanels a{at(x_hi), at(x_lo), c.T}, b0{at(g_hi), at(g_lo), c.H}, b1{at(u_hi), at(u_lo), c.H};
     const int kept_vec = c.H % 8 == 0 && reinterpret_cast<uintptr_t>(c.gate) % 32 == 0 && reinterpret_cast<uintptr_t>(c.up) % 32 == 0;
-#define NK_CASE(FUN) st = product(ctx, shape, Kp, a, b0, b1, tp, GatedDrain<FUN>{static_cast<float*>(c.y.ptr), static_cast<float*>(c.gate), static_cast<float*>(c.up), c.T, c.H, c.y.rs, c.y.cs, wide_rows(c.y), kept_vec})
+#define NK_CASE(FUN) st = product(ctx, c, shape, Kp, a, b0, b1, tp, GatedDrain<FUN>{static_cast<float*>(c.y.ptr), static_cast<float*>(c.gate), static_cast<float*>(c.up), c.T, c.H, c.y.rs, c.y.cs, wide_rows(c.y), kept_vec})
     NK_GATE_SWITCH(c.fun, NK_CASE)
 #undef NK_CASE
     *handled = true;
@@ -348,7 +349,7 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
     } else if (dx) {
         const OneDrain drain{static_cast<float*>(c.dx.ptr), c.T, c.D, c.dx.rs, c.dx.cs, wide_rows(c.dx)};
         const TcPanels a{at(a_hi), at(a_lo), c.T}, b{at(w_hi), at(w_lo), c.D};
-        if ((st = product(ctx, sx, 2 * Hp, a, b, b, tc_params(sx, c.T, 2 * Hp, at(px), ep.tickets, ctx->tma_status_dev), drain))) return st;
+        if ((st = product(ctx, c, sx, 2 * Hp, a, b, b, tc_params(sx, c.T, 2 * Hp, at(px), ep.tickets, ctx->tma_status_dev), drain))) return st;
     }
     if (dw) {
         TwoDrain drain;
@@ -362,7 +363,7 @@ int nk_gated_tc_backward(nk_ctx* ctx, const GatedCall& c, bool* handled) {
             drain.vec[b] = wide_rows(c.dw[b]);
         }
         const TcPanels a{at(x_hi), at(x_lo), c.D}, b0{at(e_at[0][0]), at(e_at[0][1]), c.H}, b1{at(e_at[1][0]), at(e_at[1][1]), c.H};
-        st = product(ctx, sw, Tp, a, b0, b1, tc_params(sw, c.D, Tp, at(pw), ep.tickets + tx_bytes / sizeof(int), ctx->tma_status_dev), drain);
+        st = product(ctx, c, sw, Tp, a, b0, b1, tc_params(sw, c.D, Tp, at(pw), ep.tickets + tx_bytes / sizeof(int), ctx->tma_status_dev), drain);
     }
     *handled = true;
     return st;

@@ -164,3 +164,22 @@ def test_gates_of_plain_products_are_right_to_the_last_bit(device, fun):
             for i in range(2):
                 same(rows[0].gradient.numpy()[i], df, "dWg")
                 same(rows[1].gradient.numpy()[i], f, "dWu")
+
+
+@pytest.mark.parametrize("one_sign", [False, True], ids=["normal", "one_sign"])
+@pytest.mark.parametrize("size", [(2, 1024, 1024), (24, 515, 900), (60, 512, 512), (150, 256, 300), (200, 64, 128), (200, 256, 300), (1023, 64, 64)], ids=str)
+def test_gated_small_products_are_as_close_as_multiply_adds(device, size, one_sign):
+    """Below 2^24 multiply-adds `@` uses those, which are 1e-7 sqrt(K / 64) off (2-norm). With weights [1, 0, 0, ...] for the gate, x of ones in its
+    first column and the gate `idy`, y = x @ wu, dwu = x^T @ e and dx = e @ wu^T (but for its first column). 3xTF32 itself: the low parts are rounded to 2^-23 of a
+    value and 2^-22 is dropped, 1e-7; accumulations in chunks of 64 terms at most lose 2e-7 of a sum of one sign, as derived above: 3e-7."""
+    t, d, h = size
+    rng = np.random.default_rng(57)
+    draw = (lambda *s: rng.uniform(0.5, 1.5, s).astype(np.float32)) if one_sign else (lambda *s: rng.standard_normal(s).astype(np.float32))
+    x, wg, wu, e = draw(t, d), np.zeros((d, h), np.float32), draw(d, h), draw(t, h)
+    x[:, 0], wg[0] = 1, 1
+    tx, tg, tu = (put(device, a).set_rqs_gradient(True) for a in (x, wg, wu))
+    y = tx.gated(tg, tu, "idy")
+    y.backward(put(device, e))
+    X, U, E = (a.astype(np.float64) for a in (x, wu, e))
+    for name, got, want in (("y", y.numpy(), X @ U), ("dwu", tu.gradient.numpy(), X.T @ E), ("dx", tx.gradient.numpy()[:, 1:], (E @ U.T)[:, 1:])):
+        assert np.linalg.norm(got - want) < 3e-7 * np.linalg.norm(want), (name, np.linalg.norm(got - want) / np.linalg.norm(want))
