@@ -437,7 +437,7 @@ nk_conv_tc_kernel(const __grid_constant__ TcMaps<Drain::DUAL> maps, const __grid
             float sum[EC];
             for (int kb0 = kb_begin; kb0 < kb_end && ok; kb0 += p.chunk, ch++) {
                 const int b = ch & 1;
-                ok = wait_or_abort(&acc_full[b], (unsigned(ch) >> 1) & 1u);
+                ok = __all_sync(0xffffffffu, wait_or_abort(&acc_full[b], (unsigned(ch) >> 1) & 1u));   // the lanes go on, or leave, together
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t src = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(b) * BN + uint32_t(quarter) * (DUAL ? EC / 2 : EC);
