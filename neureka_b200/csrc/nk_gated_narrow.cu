@@ -40,6 +40,8 @@ struct NarrowCall {
     int chunk;                 // units between two readings of the accumulators, at least 1
     int64_t total;             // units of all tiles
     int64_t Kq;                // SUM: columns of a panel per weight, a multiple of a unit
+    const float *x_hi, *x_lo;  // the tokens' panels, [T][pitch], hi and lo; SUM: the second weight's from Kq on
+    int64_t pitch;
     float* parts;              // [CTA][2][NB][NT][128]
     int* tickets;              // [tiles]
     int* status;
@@ -89,6 +91,34 @@ __device__ __forceinline__ void nw_ld8(uint32_t taddr, float (&v)[8]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 }
 __device__ __forceinline__ void nw_sync() { asm volatile("bar.sync 1, 512;\n" ::: "memory"); }   // the converters
+
+// Sums that came out as NaN because of an infinity (tc_again says how), taken again by F32 multiply-adds: a whole warp, token t, four columns from n on per lane, whose
+// sums are res[0..3] and (two products) res[second + 0..3].
+template <bool SUM>
+__device__ __noinline__ void nw_again(const NarrowCall& p, float* res, int second, int64_t t, int64_t n) {
+    const int lane = threadIdx.x & 31;
+    const float *hi = p.x_hi + t * p.pitch, *lo = p.x_lo + t * p.pitch;
+    bool found = false;   // a NaN of the token's own spoils all its sums
+    for (int64_t k = lane; k < (SUM ? p.Kq + p.K : p.K); k += 32) found = found || hi[k] != hi[k];
+    if (__any_sync(0xffffffffu, found)) return;
+    for (int i = 0; i < (SUM ? 4 : 8); i++) {   // sum by sum: what lives across the call in the caller's registers counts for more than the time of such calls
+        float* at = res + (i & 3) + (i >> 2) * second;
+        const int64_t c = n + (i & 3);
+        const bool lost = c < p.N && *at != *at;
+        if (!__any_sync(0xffffffffu, lost)) continue;
+        float v = 0.0f;
+        for (int b = SUM ? 0 : i >> 2; b < (SUM ? 2 : (i >> 2) + 1); b++) {
+            const GatedMatrix& w = p.w[b];
+            const float *column = static_cast<const float*>(w.ptr) + (lost ? c : 0) * w.cs, *x_hi = hi + (SUM && b ? p.Kq : 0), *x_lo = lo + (SUM && b ? p.Kq : 0);
+            for (int64_t k0 = 0; k0 < p.K && __any_sync(0xffffffffu, lost && v == v); k0 += 64) {   // (NaN it is, else)
+                const int kc = p.K - k0 < 64 ? int(p.K - k0) : 64;
+#pragma unroll 4
+                for (int k = 0; k < kc; k++) v = fmaf(x_hi[k0 + k] + x_lo[k0 + k], column[(k0 + k) * w.rs], v);
+            }
+        }
+        if (lost) *at = v;
+    }
+}
 
 template <int NT, bool SUM, int LAYOUT>
 __global__ void __launch_bounds__(NW_THREADS, 1)
@@ -401,7 +431,15 @@ nk_gated_narrow_kernel(const __grid_constant__ CUtensorMap map_hi, const __grid_
                 for (int k = 0; k < VE; k++) {
                     const int e = e0 + k * 2048;
                     const int64_t t = t0 + (e >> 7), n = n0 + (e & 127);
-                    if (t >= p.T) break;
+                    if (t >= p.T) break;   // (a warp has one token)
+                    bool lost = false;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) lost = lost || (n + j < p.N && (res[e + j] != res[e + j] || (!SUM && res[C::RES / 2 + e + j] != res[C::RES / 2 + e + j])));
+                    if (__any_sync(0xffffffffu, lost)) {
+                        if (!waited) asm volatile("griddepcontrol.wait;\n" ::: "memory");   // for the panels
+                        waited = true;
+                        nw_again<SUM>(p, res + e, C::RES / 2, t, n);
+                    }
                     float* o = static_cast<float*>(p.out.ptr) + t * p.out.rs + n * p.out.cs;
 #pragma unroll 1
                     for (int j = 0; j < 4 && n + j < p.N; j++) {
@@ -465,7 +503,7 @@ int narrow_grid(const nk_ctx* ctx, const NarrowCall& p) {
 size_t narrow_part_bytes(const nk_ctx* ctx, const NarrowCall& p, bool sum) { return size_t(narrow_grid(ctx, p)) * 2 * (sum ? 1 : 2) * narrow_tokens(p.T) * 128 * 4; }
 
 template <int NT, bool SUM, int LAYOUT>
-int narrow_launch(nk_ctx* ctx, const NarrowCall& p, const float* hi, const float* lo, int64_t cols) {
+int narrow_launch(nk_ctx* ctx, NarrowCall p, const float* hi, const float* lo, int64_t cols) {
     using C = NarrowCfg<NT, SUM>;
     CUtensorMap map_hi, map_lo;
     if (nk_tma_encode_2d_f32(hi, uint64_t(p.T), uint64_t(cols), uint64_t(cols) * 4, 16, NT, 2, &map_hi) ||
@@ -473,6 +511,9 @@ int narrow_launch(nk_ctx* ctx, const NarrowCall& p, const float* hi, const float
         return nk_fail(ctx, NK_ERR_CUDA, "nk_gated: the driver has no tensor-map encoder");
     auto* kern = nk_gated_narrow_kernel<NT, SUM, LAYOUT>;
     NK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    p.x_hi = hi;
+    p.x_lo = lo;
+    p.pitch = cols;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(unsigned(narrow_grid(ctx, p)));

@@ -4,7 +4,7 @@
 // 3xTF32. A TF32 operand keeps 11 significant bits, an F32 value 24. Every operand element v is split once into
 // hi = tf32(v) (round to nearest) and lo = tf32(v - hi) (v - hi is exact in F32), and the product sum is evaluated as
 // sum(lo_a*hi_b) + sum(hi_a*lo_b) + sum(hi_a*hi_b) with F32 accumulation in tensor memory: the dropped lo*lo term and
-// the rounding of lo are below 2^-21 of |a||b| per term, inside the 1e-5 * sum|a||b| tolerance of the path.
+// the rounding of lo are below 2^-21 of |a||b| per term, inside the 1e-5 * sum|a||b| tolerance of the path. Sums with infinite operands: tc_again.
 //
 // Two shapes of the kernel, chosen by estimated time (tc_shape):
 //   * pairs of CTAs (cta_group::2), tile 256 x 256: each CTA stages 128 rows of A and 128 of B, 32 KiB per 16 k where a lone
@@ -231,6 +231,8 @@ struct TcParams {
     int64_t units;                 // tiles * splits; unit u is part u % splits of tile u / splits
     int splits, kb_per;            // k blocks per part
     int chunk;                     // k blocks per accumulation chunk
+    const float *a[2], *b[4];      // the panels, hi and lo of A and of each B, rows of Kp: what tc_again reads
+    int64_t N, Kp;                 // rows of B
     float* parts;                  // splits > 1: [tile][part][warp of 16][columns / 4][32 rows x 4]
     int* tickets;                  // splits > 1: [tile][warp of 16]
     int* status;                   // host-mapped word, set non-zero when a bounded wait ran out
@@ -272,6 +274,63 @@ struct TcPlainDrain {
         }
     }
 };
+
+// An infinity's lo is 0 and its products with the other operand's low bits are NaN (0) or of either sign, so three products give NaN where the sum of
+// hi + lo is infinite. Sums that come out as NaN are taken again, by F32 multiply-adds over the panels: sum[j] of a thread is that of its row m and column n0 + j
+// (two B operands: the first half of the second one's). Called by a whole warp, which shares the work of each; rows and columns with a NaN
+// of their own, which spoil all their sums, are found first.
+template <int EC, bool DUAL>
+__device__ __noinline__ void tc_again(const TcParams& p, float* sum, int64_t m, int64_t n0) {
+    constexpr int COLS = DUAL ? EC / 2 : EC;
+    const int lane = threadIdx.x & 31;
+    auto has_nan = [&](const float* row) {
+        bool found = false;
+        for (int64_t k = lane * 4; k - lane * 4 < p.Kp && !found; k += 128) {
+            const float4 v = k < p.Kp ? *reinterpret_cast<const float4*>(row + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            found = __any_sync(0xffffffffu, v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w);
+        }
+        return found;
+    };
+    auto columns = [&](int j) { return n0 + j % COLS < p.N; };
+    bool mine = false;
+    for (int j = 0; j < EC; j++) mine = mine || (columns(j) && sum[j] != sum[j]);
+    mine = mine && m < p.M;
+    for (unsigned rows = __ballot_sync(0xffffffffu, mine); rows; rows &= rows - 1) {
+        const int r = __ffs(int(rows)) - 1;
+        const bool spoilt = has_nan(p.a[0] + __shfl_sync(0xffffffffu, m, r) * p.Kp);
+        if (lane == r) mine = !spoilt;
+    }
+    for (int j = 0; j < EC; j++) {
+        unsigned rows = __ballot_sync(0xffffffffu, mine && columns(j) && sum[j] != sum[j]);
+        if (!rows) continue;
+        const int which = DUAL ? 2 * (j / COLS) : 0;
+        const int64_t column = (n0 + j % COLS) * p.Kp;
+        const float *b_hi = p.b[which] + column, *b_lo = p.b[which + 1] + column;
+        if (has_nan(b_hi)) continue;
+        for (; rows; rows &= rows - 1) {
+            const int r = __ffs(int(rows)) - 1;
+            const int64_t row = __shfl_sync(0xffffffffu, m, r) * p.Kp;
+            const float *a_hi = p.a[0] + row, *a_lo = p.a[1] + row;
+            float v = 0.0f;
+            bool done = false;
+            for (int64_t k0 = 0; k0 < p.Kp && !done; k0 += 128) {
+                const int64_t k = k0 + lane * 4;
+                if (k < p.Kp) {   // (Kp is a multiple of 16)
+                    const float4 x = *reinterpret_cast<const float4*>(a_hi + k), y = *reinterpret_cast<const float4*>(a_lo + k);
+                    const float4 z = *reinterpret_cast<const float4*>(b_hi + k), w = *reinterpret_cast<const float4*>(b_lo + k);
+                    v = fmaf(x.x + y.x, z.x + w.x, v);
+                    v = fmaf(x.y + y.y, z.y + w.y, v);
+                    v = fmaf(x.z + y.z, z.z + w.z, v);
+                    v = fmaf(x.w + y.w, z.w + w.w, v);
+                }
+                done = __any_sync(0xffffffffu, v != v);   // (NaN it is)
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane == r) sum[j] = v;
+        }
+    }
+}
 
 template <int CG, int BN, class Drain>
 __global__ void __launch_bounds__(TC_THREADS, 1)
@@ -485,6 +544,17 @@ nk_conv_tc_kernel(const __grid_constant__ TcMaps<Drain::DUAL> maps, const __grid
                     }
                 }
             }
+            bool lost = false;
+#pragma unroll
+            for (int j = 0; j < EC; j++) lost = lost || sum[j] != sum[j];
+            if (__any_sync(0xffffffffu, lost)) {
+                float again[EC];
+#pragma unroll
+                for (int j = 0; j < EC; j++) again[j] = sum[j];
+                tc_again<EC, DUAL>(p, again, m, n0);
+#pragma unroll
+                for (int j = 0; j < EC; j++) sum[j] = again[j];
+            }
             drain.store(m, n0, sum);
         }
     }
@@ -554,7 +624,7 @@ struct TcPanels {
 };
 // -1: there is no tensor-map encoder
 template <int CG, int BN, class Drain>
-int tc_launch(nk_ctx* ctx, const char* name, int64_t Kp, const TcPanels& A, const TcPanels& B0, const TcPanels& B1, const TcParams& tp, const Drain& drain) {
+int tc_launch(nk_ctx* ctx, const char* name, int64_t Kp, const TcPanels& A, const TcPanels& B0, const TcPanels& B1, TcParams tp, const Drain& drain) {
     using C = TcCfg<CG, BN>;
     constexpr bool DUAL = Drain::DUAL;
     TcMaps<DUAL> maps;
@@ -567,6 +637,10 @@ int tc_launch(nk_ctx* ctx, const char* name, int64_t Kp, const TcPanels& A, cons
     if constexpr (DUAL) {
         if (encode(B1, B_BOX, maps.b + 2)) return -1;
     }
+    tp.a[0] = A.hi; tp.a[1] = A.lo;
+    tp.b[0] = B0.hi; tp.b[1] = B0.lo; tp.b[2] = B1.hi; tp.b[3] = B1.lo;
+    tp.N = B0.rows;
+    tp.Kp = Kp;
     auto* kern = nk_conv_tc_kernel<CG, BN, Drain>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     if (e != cudaSuccess) return nk_cuda_fail(ctx, e, "cudaFuncSetAttribute(nk_conv_tc_kernel)");

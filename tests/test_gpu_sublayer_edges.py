@@ -183,3 +183,77 @@ def test_gated_small_products_are_as_close_as_multiply_adds(device, size, one_si
     X, U, E = (a.astype(np.float64) for a in (x, wu, e))
     for name, got, want in (("y", y.numpy(), X @ U), ("dwu", tu.gradient.numpy(), X.T @ E), ("dx", tx.gradient.numpy()[:, 1:], (E @ U.T)[:, 1:])):
         assert np.linalg.norm(got - want) < 3e-7 * np.linalg.norm(want), (name, np.linalg.norm(got - want) / np.linalg.norm(want))
+
+
+# ---- operands that are not finite ----------------------------------------------------------------------------------------------------
+def product(a, b):
+    """a @ b in F64, from products of finite matrices alone: which terms of a sum are infinite, of which sign, or no number, counted"""
+    def count(p, q):
+        return p.astype(np.float64) @ q.astype(np.float64) > 0
+    (ai, ap, an, a0), (bi, bp, bn, b0) = ((np.isinf(m), m > 0, m < 0, m == 0) for m in (a, b))
+    plus = count(ai & ap, bp) | count(ai & an, bn) | count(ap, bi & bp) | count(an, bi & bn)
+    minus = count(ai & ap, bn) | count(ai & an, bp) | count(ap, bi & bn) | count(an, bi & bp)
+    none = np.isnan(a).any(1)[:, None] | np.isnan(b).any(0)[None] | count(ai, b0) | count(a0, bi)
+    c = np.where(np.isfinite(a), a, 0).astype(np.float64) @ np.where(np.isfinite(b), b, 0).astype(np.float64)
+    return np.where(none | (plus & minus), np.nan, np.where(plus, np.inf, np.where(minus, -np.inf, c)))
+
+
+def same_kind(got, want, what):
+    """NaN where the plain form has NaN, the same infinity where it has one, finite elsewhere"""
+    def kind(a):
+        return np.where(np.isnan(a), 9, np.where(np.isinf(a), np.sign(np.where(np.isnan(a), 0, a)), 0)).astype(int)
+    a, b = kind(got), kind(want)
+    assert np.array_equal(a, b), f"{what}: {int((a != b).sum())} of {a.size} of another kind"
+
+
+# one token; some; a lone CTA's tiles, their k split, pairs; narrow sides
+INFINITE = [(1, 96, 128), (2, 96, 128), (8, 100, 72), (24, 300, 257), (24, 4100, 136), (64, 130, 260), (150, 96, 200), (300, 260, 130), (300, 2100, 130), (2600, 300, 1100), (300, 30, 500)]
+
+
+@pytest.mark.parametrize("turned", [False, True], ids=["", "turned"])
+@pytest.mark.parametrize("size", INFINITE, ids=str)
+def test_gated_of_infinite_operands(device, size, turned):
+    """An infinity times a finite value is an infinity, whatever the other value's low bits are and however many tokens there are."""
+    t, d, h = size
+    rng = np.random.default_rng(55)
+
+    def draw(*shape):   # values whose low bits are zero, positive or negative, in turn, and a few zeros
+        a = rng.standard_normal(shape).astype(np.float32)
+        a = np.where(rng.random(shape) < 0.3, np.round(a * 4) / 4, a)
+        return np.where(rng.random(shape) < 0.01, 0, a).astype(np.float32)
+
+    x, wg, wu, e = draw(t, d), draw(d, h), draw(d, h), draw(t, h)
+    for place in ("x", "w", "both", "e"):
+        X, G, U, E = x.copy(), wg.copy(), wu.copy(), e.copy()
+        if place in ("x", "both"):
+            X[t // 2, d // 3] = np.inf
+            X[t - 1, d - 1] = -np.inf
+        if place in ("w", "both"):
+            G[d // 2, h // 3] = -np.inf
+            U[d - 1, h - 1] = np.inf
+        if place == "e":
+            E[t // 2, h // 2] = np.inf
+            E[t - 1, 0] = -np.inf
+        tx, tg, tu = (put(device, a, "turned" if turned and k else "dense").set_rqs_gradient(True) for k, a in enumerate((X, G, U)))
+        y = tx.gated(tg, tu, "idy")
+        y.backward(put(device, E))
+        with np.errstate(invalid="ignore"):
+            g, u = product(X, G), product(X, U)
+            dg, du = E * u, E * g
+            same_kind(y.numpy(), g * u, f"y {place}")
+            same_kind(tx.gradient.numpy(), product(dg, G.T) + product(du, U.T), f"dx {place}")
+            same_kind(tg.gradient.numpy(), product(X.T, dg), f"dwg {place}")
+            same_kind(tu.gradient.numpy(), product(X.T, du), f"dwu {place}")
+
+
+@pytest.mark.parametrize("size", [(256, 256, 300), (300, 4100, 70), (1100, 300, 1030)], ids=str)
+def test_matrix_product_of_infinite_operands(device, size):
+    """... and so for `@`, whose large products are computed the same way"""
+    m, k, n = size
+    rng = np.random.default_rng(56)
+    a, b = (np.where(rng.random(s) < 0.3, 0.5, rng.standard_normal(s)).astype(np.float32) for s in ((m, k), (k, n)))
+    a[m // 2, k // 3], a[m - 1, k - 1], b[k // 2, n // 3], a[3, 5] = np.inf, -np.inf, np.inf, np.nan
+    b[k // 3, 7] = 0
+    got = (put(device, a) @ put(device, b)).numpy()
+    with np.errstate(invalid="ignore"):
+        same_kind(got, product(a, b), "a @ b")
