@@ -426,7 +426,7 @@ nk_gated_narrow_kernel(const __grid_constant__ CUtensorMap map_hi, const __grid_
                     for (int k = 0; k < VE * C::NB; k++) *reinterpret_cast<float4*>(res + e0 + k * 2048) = v[k];   // (this thread's own elements)
                 }
             }
-            if (finish && !*abort_word) {
+            if (__all_sync(0xffffffffu, finish && !*abort_word)) {   // (one answer per warp)
 #pragma unroll 1
                 for (int k = 0; k < VE; k++) {
                     const int e = e0 + k * 2048;
