@@ -232,7 +232,9 @@ int nk_fused_run_grad(nk_ctx* ctx, nk_fused* f, int32_t rank, nk_buf* grad, cons
 
 /* ---- a feed-forward sub-layer: layer norm, dropout, the gated block (no counterpart in the reference) ----
  * F32 and F64. Operands are views like everywhere else; each call takes what it needs beside them from the device's memory pool in the
- * order of ctx's stream and gives it back, so that calls on several contexts, or captured into several graphs, share nothing. A drain's
+ * order of ctx's stream and gives it back (layer norm's backward pass: some sums per row and multiprocessor; nk_gated on the tensor cores: 8 bytes
+ * per element of src and weights, nk_gated_grad there 32 bytes per element of [T, H] and 8 per element of src and weights: 1.3 GB for T = 4096, D = 2048,
+ * H = 8192; NK_ERR_OOM where there is no room), so that calls on several contexts, or captured into several graphs, share nothing. A drain's
  * elements must be distinct (no virtual drain), and a drain may not overlap another operand unless said otherwise. */
 
 /* Layer norm over the last dim (n = its extent; a row = the elements that share all other indices): mu = mean(src), v = mean((src - mu)^2),

@@ -272,7 +272,7 @@ template <class T, int TOK, bool TURNED, bool VEC, bool SUM>
 int few_launch(nk_ctx* ctx, FewCall p) {
     constexpr int COLS = 32 * few_v<T>;
     constexpr size_t smem = sizeof(T) * TOK * ((SUM ? 2 : 1) * FEW_K + (SUM ? 1 : 2) * COLS);
-    // k is split until there are about four CTAs per SM, at most eight ways (a portable cluster)
+    // k is split until there are at least three CTAs per SM (it doubles, so up to six), at most eight ways (a portable cluster)
     const int64_t tiles = (p.N + COLS - 1) / COLS, pieces = (p.K + FEW_SLICE - 1) / FEW_SLICE;
     int split = 1;
     while (split < 8 && split < pieces && tiles * split < int64_t(ctx->prop.multiProcessorCount) * 3) split *= 2;

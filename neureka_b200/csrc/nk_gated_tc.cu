@@ -5,7 +5,7 @@
 // elements and stores f(g) * u (and g and u, where a backward pass follows) straight from its registers.
 // Backward: nk_gated_errors_split_kernel reads e, g and u once and leaves dg = e u f'(g) and du = e f(g) as panels in both directions they are needed in:
 // [T, dg | du] for dx = [dg | du] [Wg | Wu]^T, one product over 2 H, and [H, T] each for dWg | dWu = x^T [dg | du], the product with two B
-// operands again.
+// operands again. These panels are 32 bytes per element of T x H (dx or dW alone: 16), those of the forward pass 8 per element of x and the weights.
 #include "nk_gated.cuh"
 #include "nk_tc.cuh"
 

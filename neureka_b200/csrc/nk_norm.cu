@@ -154,7 +154,7 @@ __device__ __forceinline__ void norm_results(T* y, const T* gain, const T* shift
 
 // ---- rows that a group of lanes, a CTA or a cluster holds in registers ---------------------------------------------------------------
 // One pass over the data: x stays in registers between the mean, the variance and the result. Short rows, and calls with too few rows to keep teams
-// with rings busy (below), which the latency of a row bounds: 1 x 4096 5.4 us, 1000 x 777 forward 8.2 us; 400000 x 64 69 us (3.0 TB/s).
+// with rings busy (below), which the latency of a row bounds: 1 x 4096 5.4 us, 1000 x 777 forward 8.2 us; 400000 x 64 69 us (3.0 TB/s: a row per group in flight, its two sums one after the other).
 
 // CTAs per SM that the registers have to leave room for: fewer cost more than a few spilled words (200000 x 200 by two of them 140 us, by three 109)
 template <class T, int W, int E>
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(256) nk_norm_grad_lanes_kernel(T* out, const T
 // A team of TW warps takes a row at a time. Its rows arrive in shared memory by cp.async.bulk, several ahead, so that the memory is kept busy
 // through the reductions; the copies need nothing but 16-byte boundaries around a row, so rows that start anywhere cost no more than aligned ones
 // (element-wise loads of rows into registers reached a third of the memory's rate). Forward and backward: 16384 x 4096 98 and 153 us (5.5 and 5.3
-// TB/s, bound by the memory), 8192 x 8192 92 / 162, 30000 x 1001 47 / 81; rows that a cluster shares wait for its slowest CTA: 2000 x 20000 162 / 227
+// TB/s, bound by the memory), 8192 x 8192 92 / 161, 30000 x 1001 47 / 81; rows that a cluster shares wait for its slowest CTA: 2000 x 20000 162 / 227
 // (2 TB/s). A row's 16-byte boundaries may lie outside its buffer at
 // the buffer's ends: such a row is read by plain loads.
 constexpr int STREAM_WARPS = 16, STREAM_THREADS = 512, STREAM_SMEM = 200 * 1024, STREAM_STAGES = 8;
@@ -946,7 +946,8 @@ bool norm_vec(const NormPlan& p, int t, const T* base) {
     return true;
 }
 
-// one resident wave at most; a cluster's CTAs lie side by side
+// at most per_sm CTAs per SM (the backward calls' are resident at once, since each leaves its column sums; the forward calls' are several waves, so that the
+// hardware evens out what rows take); a cluster's CTAs lie side by side
 template <class... A>
 int norm_launch(nk_ctx* ctx, const char* name, void (*kern)(A...), int64_t rows, int threads, int cluster, int per_sm, A... args) {
     int64_t units = int64_t(ctx->prop.multiProcessorCount) * per_sm / cluster;
@@ -971,8 +972,8 @@ int norm_launch(nk_ctx* ctx, const char* name, void (*kern)(A...), int64_t rows,
 template <class T> constexpr int norm_e() { return 128 / int(sizeof(T)); }
 
 // Rows by bulk copies: at least two of them for every team, running along memory, and long: up to 256 elements on 16-byte boundaries a group of lanes
-// per row is as fast or faster (200000 x 200: forward 105 us against 100, backward 139 against 157; 200000 x 203, which has no such
-// boundaries: 127 against 102 and 237 against 152).
+// per row is as fast or faster (200000 x 200: forward 109 us against 106, backward 133 against 158; 200000 x 203, which has no such
+// boundaries: 139 against 107 and 229 against 152).
 template <class T> constexpr int stream_e() { return 64 / int(sizeof(T)); }
 struct StreamShape {
     int team, cluster, stages, stage_bytes, cols, grid;

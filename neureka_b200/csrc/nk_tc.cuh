@@ -21,6 +21,8 @@
 // sixteen epilogue warps add every finished chunk into per-thread F32 running sums with ordinary round-to-nearest adds
 // while the next chunk's products already run into the other accumulator. The running sums of a tile (a quarter of its
 // columns per thread) go to the drain after its last chunk.
+// Eighteen warps leave 96 registers a thread (five warps share a register file). A thread of the pair form holds 64 sums, and its store spills: 4 bytes a
+// thread for the plain drain, 200 to 680 for the block's, once per tile; the lone form fits.
 // Every mbarrier wait is bounded (nk_mbar_wait_bounded); on expiry the waiter raises the CTA's abort word and the
 // host-visible status, all roles leave their loops, outstanding copies and tensor-core work are waited for (bounded),
 // tensor memory is released and the kernel returns; the host then reports NK_ERR_TIMEOUT.
