@@ -8,8 +8,8 @@
 // (nk_gated_tc.cu does, where a panel is used by many tiles). Here a warp brings 32 columns x 16 k into shared memory (cp.async, two or three
 // such patches ahead: loads into registers, two ahead, left the memory at a third of its rate), splits them in registers and stores hi
 // and lo into tensor memory, from where tcgen05.mma takes its A operand. The tokens' panels are split before (they are small) and come by TMA.
-// What is left is the stream of weights: 4 bytes per element against 6 multiply-adds per token. 16 tokens x 4096 x 8192 69 us, where the weights' bytes take
-// 41; 64 tokens 85; 24 x 2048 x 5461 37 us (14): bound by the issue of the converters (split, store) and, from 64 tokens on, by the products.
+// What is left is the stream of weights: 4 bytes per element against 6 multiply-adds per token. 16 tokens x 4096 x 8192 64 us, where the weights' bytes take
+// 41; 64 tokens 80; 24 x 2048 x 5461 38 us (14): bound by the issue of the converters (split, store) and, from 64 tokens on, by the products.
 //
 // Roles, 18 warps: 0..15 converters in two groups, warp 16 fetches the tokens' panels, warp 17 issues the products. A stage is 32 k of both weights
 // (SUM: 64 k of one); every converter splits 32 columns x 16 k of it, warp w for lanes 32 (w % 4) of the tile. Tensor memory: three (two)
@@ -553,7 +553,7 @@ int narrow(nk_ctx* ctx, const NarrowCall& p, const float* hi, const float* lo, i
 }  // namespace
 
 bool nk_gated_narrow(const nk_ctx* ctx, const GatedCall& c) {
-    // Up to three tiles of 64 tokens: every tile reads the weights again (64 tokens 84 us at 4096 x 8192), where panels of them (nk_gated_tc.cu) cost
+    // Up to three tiles of 64 tokens: every tile reads the weights again (64 tokens 80 us at 4096 x 8192), where panels of them (nk_gated_tc.cu) cost
     // their split, 150 us there, and 1.1 us per token.
     if (c.T > 192 || c.D < 16 || c.H < 16) return false;
     const int64_t most = int64_t(1) << 30;

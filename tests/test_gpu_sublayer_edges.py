@@ -8,7 +8,7 @@ import pytest
 import sublayer as S
 from neureka_b200 import _lib as L
 from neureka_b200 import functions as F
-from test_gpu_sublayer import put
+from test_gpu_sublayer import put, sub_layer_calls
 
 pytestmark = pytest.mark.gpu
 
@@ -257,3 +257,55 @@ def test_matrix_product_of_infinite_operands(device, size):
     got = (put(device, a) @ put(device, b)).numpy()
     with np.errstate(invalid="ignore"):
         same_kind(got, product(a, b), "a @ b")
+
+
+def test_split_sums_and_sums_taken_again_captured_and_replayed(device):
+    """What takes memory for the length of a call, or looks at its sums again, does so under capture as well: a narrow block of many tokens, and infinities."""
+    import torch
+    for case, place in (((np.float32, 20000, 40, 48), None), ((np.float32, 300, 260, 515), (7, 9)), ((np.float32, 24, 300, 257), (3, 5))):
+        (x, wg), results, run, raw = sub_layer_calls(device.ctx, *case)
+        stream = torch.cuda.ExternalStream(L.lib.nk_stream(device.ctx))
+        run()
+        device.sync()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+            run()
+        for _ in range(2):
+            wg.mul_(-1.25)
+            if place is not None:
+                wg[place] = float("inf")
+            torch.cuda.synchronize()
+            run()
+            device.sync()
+            want = [r.clone() for r in results]
+            for r in results:
+                r.fill_(-7)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(torch.nan_to_num(a, nan=-3.5), torch.nan_to_num(b, nan=-3.5)) and torch.equal(a.isnan(), b.isnan()) for a, b in zip(results, want))
+            assert bool(torch.isinf(results[1]).any()) == (place is not None)
+
+
+def test_two_contexts_split_long_sums_at_once(device):
+    import ctypes as C
+    import torch
+    second = C.c_void_p()
+    L.check(L.lib.nk_device_open(device.ordinal, C.byref(second)))
+    try:
+        sides = []
+        for ctx in (device.ctx, second):
+            _, results, run, raw = sub_layer_calls(ctx, np.float32, 30000, 24, 40)
+            run()
+            L.check(L.lib.nk_sync(ctx), ctx)
+            sides.append((results, [r.clone() for r in results], run, raw))
+        for _ in range(10):
+            for _, _, run, _ in sides:
+                run()
+        torch.cuda.synchronize()
+        for results, want, _, _ in sides:
+            assert all(torch.equal(a, b) for a, b in zip(results, want))
+        del sides, results, want, run, raw
+    finally:
+        L.lib.nk_device_close(second)
